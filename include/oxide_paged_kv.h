@@ -403,6 +403,39 @@ void qk_norm_rope_and_cache(void* q_out, void* k_out, const void* qkv, int64_t q
                             int64_t num_kv_heads, int64_t head_dim, int dtype, void* stream);
 
 /*
+ * qk_norm_rope_and_cache with positions on several axes (time, height and width of
+ * image and video tokens).  No reference counterpart: its rotation
+ * (crates/vllm-oxide/src/layers/rope.rs:133-163) has one position per token.
+ * Frequency j (0 <= j < head_dim / 2, the pair x[j], x[j + head_dim / 2]) is turned by
+ * row positions[axis(j)][t] of the cos / sin table.
+ *
+ *   positions   int32 [num_axes, num_tokens]; values outside [0, max_position) are
+ *               clamped into it
+ *   num_axes    1 .. 4
+ *   sections    HOST array int32 [num_axes], read during the call: the number of
+ *               frequencies of each axis, together head_dim / 2
+ *   interleaved 0: the axes hold runs of frequencies, sections[0] of axis 0 first, then
+ *               sections[1] of axis 1, ...; 1: they are dealt in turn, axis a >= 1 holds
+ *               j = a, a + A, a + 2 A, ... (sections[a] of them, A = num_axes) and axis 0
+ *               the others; a last such j past head_dim / 2 is an invalid argument
+ *   num_slots   rows of the caches (num_blocks * block_size); tokens with a slot outside
+ *               [0, num_slots) are not appended
+ *
+ * Other arguments as for qk_norm_rope_and_cache.  Rounding differs from it: norm,
+ * weight and rotation are computed in fp32 throughout and rounded once to the dtype
+ * (the single-axis entry rounds after each of the three, as the reference does), so with
+ * equal positions on all axes the two agree within those roundings, not bit for bit.
+ * Supported: f16/bf16, head_dim 64 or 128.
+ */
+void qk_norm_mrope_and_cache(void* q_out, void* k_out, const void* qkv, int64_t qkv_row_stride,
+                             const void* q_norm_weight, const void* k_norm_weight, double eps,
+                             const float* cos_sin_cache, int64_t max_position, const int32_t* positions,
+                             int64_t num_axes, const int32_t* sections, int interleaved, void* key_cache,
+                             void* value_cache, int64_t num_slots, const int64_t* slot_mapping,
+                             int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                             int dtype, void* stream);
+
+/*
  * Host helper: fills `cache` (host memory, max_position * rotary_dim floats)
  * with RotaryEmbedding's cos_sin_cache (crates/vllm-oxide/src/layers/rope.rs:50-83):
  * row t = [cos(t f_i) | sin(t f_i)], f_i = 1 / base^(2i / rotary_dim), fp32.
@@ -423,6 +456,99 @@ int oxide_rope_cos_sin_cache(float* cache, int64_t max_position, int64_t rotary_
 void build_decode_metadata_device(const uint32_t* context_lens, const int32_t* block_table,
                                   int64_t max_blocks_per_seq, int64_t batch, int64_t block_size,
                                   uint32_t* cu_seqlens_k, int64_t* slot_mapping, void* stream);
+
+/*
+ * Metadata of a whole step -- prompts, chunks of prompts and single tokens mixed --
+ * from the requests' lengths, block tables extended on the device.  The reference does
+ * this on the host (crates/vllm-oxide/src/engine/mod.rs:160-196, metadata.rs:49-80,
+ * kv_cache_manager.rs:115-135, block_pool.rs:96-369); build_decode_metadata_device
+ * covers a decode step whose tables are complete.
+ *
+ * With C = context_lens[b] (tokens in the cache), Q = query_lens[b] (new ones, 0 = idle),
+ * P = block_size, W = max_blocks_per_seq:
+ *   cu_seqlens_q, cu_seqlens_k   uint32 [batch + 1]: prefix sums of Q and of C + Q
+ *   held = min(W, ceil(C / P)), need = min(W, ceil((C + Q) / P))
+ *   cu_new_blocks                uint32 [batch + 1]: prefix sums of need - held
+ *   block_table                  int32 [batch, W], in and out: entries < held are read;
+ *       request b takes its need - held blocks from free_blocks[cu_new_blocks[b] ...],
+ *       in order, into entries held .. need - 1, if the list reaches that far
+ *       (cu_new_blocks[b + 1] <= num_free_blocks); otherwise it takes none.  Entries
+ *       outside these are left as they are.
+ *   slot_mapping                 int64 [num_tokens]: row cu_seqlens_q[b] + i is token
+ *       p = C + i: block_table[b][p / P] * P + p % P, or -1 where p / P >= W or the
+ *       block was not handed out
+ *   positions                    int32 [num_axes, num_tokens] or NULL: p +
+ *       position_offsets[b] on every axis (position_offsets int32 [batch] or NULL = 0)
+ * Rows from cu_seqlens_q[batch] on (a captured step's spare rows) get slot -1 and
+ * position 0; tokens past num_tokens get no row.  Sums of lengths beyond 32 bits wrap.
+ * batch <= 65535, batch * W < 2^31.  One small launch up to 1024 requests, two beyond.
+ */
+void build_step_metadata_device(const uint32_t* context_lens, const uint32_t* query_lens,
+                                const int32_t* position_offsets, int32_t* block_table,
+                                int64_t max_blocks_per_seq, const int32_t* free_blocks, int64_t num_free_blocks,
+                                int64_t batch, int64_t block_size, int64_t num_tokens, int64_t num_axes,
+                                uint32_t* cu_seqlens_q, uint32_t* cu_seqlens_k, uint32_t* cu_new_blocks,
+                                int64_t* slot_mapping, int32_t* positions, void* stream);
+
+/*
+ * Linear attention with a decay for each head, single tokens: per sequence b and kv head
+ * n, with the state S [head_dim, head_dim] (key dimension first) of slot state_slots[b],
+ *   S <- exp(log_decay[n]) S + k v^T,     out[h] = scale * q[h]^T S  for the heads h of n
+ * (query head h belongs to kv head h / (num_heads / num_kv_heads), which share a state).
+ * The state takes the place of a paged cache in layers whose context has a fixed size; no
+ * reference counterpart (every layer of its models is softmax attention,
+ * crates/vllm-oxide/src/models/qwen3.rs:141-230).
+ *
+ *   out          [batch, num_heads, head_dim], contiguous; must not overlap q, k or v
+ *   q            batch rows of [num_heads, head_dim], q_row_stride elements apart (parts
+ *                of a merged projection's rows); k, v likewise with num_kv_heads
+ *   log_decay    fp32 [num_kv_heads], 0 = no decay, -inf = no memory; values above 0 grow
+ *   state        fp32 [num_slots, num_kv_heads, head_dim, head_dim], in and out
+ *   state_slots  int32 [batch]; a slot outside [0, num_slots) skips the sequence: its
+ *                output row is left as it is.  Slots of one call must differ: for a slot
+ *                given twice, which sequence's state it ends with is not defined.
+ *
+ * q, k, v, out and state have to be 16-byte aligned and the row strides multiples of 8.
+ * Supported: f16/bf16, head_dim 64 or 128, any group.  State and sums are fp32.
+ */
+void linear_attention_decode(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,
+                             int64_t k_row_stride, int64_t v_row_stride, const float* log_decay, float* state,
+                             const int32_t* state_slots, int64_t num_slots, int64_t batch, int64_t num_heads,
+                             int64_t num_kv_heads, int64_t head_dim, float scale, int dtype, void* stream);
+
+/*
+ * Linear attention with a decay for each head over prompts: the recurrence of
+ * linear_attention_decode over the tokens of each sequence, computed in chunks.
+ *
+ *   out, q       [total_q, num_heads, head_dim] (q with q_row_stride), rows
+ *                cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1 of sequence b; k, v likewise.
+ *                Rows of no sequence are left as they are.
+ *   context_lens uint32 [batch] or NULL: where it is 0 the sequence starts from a zero
+ *                state and what its slot holds is not read; otherwise (and with NULL) it
+ *                goes on from its slot's state
+ *   state        the slot gets the state behind the last token; a sequence without tokens
+ *                leaves its slot as it is.  state_slots as for linear_attention_decode.
+ *   max_seqlen_q maximum length (larger lengths are clamped to it)
+ *   workspace    linear_attention_prefill_workspace_size(...) bytes (no initialisation
+ *                needed), with which long sequences are worked on in pieces side by side;
+ *                without one (NULL, not 16-byte aligned or too small) each sequence is
+ *                walked from its first chunk to its last, with the same results within
+ *                rounding.  Calls that share a workspace must not overlap in time.
+ *
+ * A NaN or infinity in v reaches its own token and later ones, no earlier one.
+ * Alignment, types and shapes as for linear_attention_decode.
+ */
+void linear_attention_prefill(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,
+                              int64_t k_row_stride, int64_t v_row_stride, const float* log_decay, float* state,
+                              const int32_t* state_slots, const uint32_t* context_lens,
+                              const uint32_t* cu_seqlens_q, int64_t num_slots, int64_t total_q, int64_t batch,
+                              int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_seqlen_q,
+                              float scale, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
+/* Bytes of workspace with which linear_attention_prefill works on pieces of these
+ * arguments' sequences side by side; 0 where it would not. */
+size_t linear_attention_prefill_workspace_size(int64_t total_q, int64_t batch, int64_t num_heads,
+                                               int64_t num_kv_heads, int64_t head_dim, int64_t max_seqlen_q);
 
 /*
  * paged_decode_attention_append (key, value, slot_mapping given) or

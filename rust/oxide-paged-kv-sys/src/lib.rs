@@ -405,6 +405,33 @@ extern "C" {
         stream: HipStream,
     );
 
+    /// The prologue with positions on several axes (`sections`: host array of `num_axes` frequency counts).
+    pub fn qk_norm_mrope_and_cache(
+        q_out: *mut c_void,
+        k_out: *mut c_void,
+        qkv: *const c_void,
+        qkv_row_stride: i64,
+        q_norm_weight: *const c_void,
+        k_norm_weight: *const c_void,
+        eps: f64,
+        cos_sin_cache: *const f32,
+        max_position: i64,
+        positions: *const i32,
+        num_axes: i64,
+        sections: *const i32,
+        interleaved: c_int,
+        key_cache: *mut c_void,
+        value_cache: *mut c_void,
+        num_slots: i64,
+        slot_mapping: *const i64,
+        num_tokens: i64,
+        num_heads: i64,
+        num_kv_heads: i64,
+        head_dim: i64,
+        dtype: c_int,
+        stream: HipStream,
+    );
+
     /// Host: RotaryEmbedding's fp32 cos/sin table (crates/vllm-oxide/src/layers/rope.rs:50-83).
     pub fn oxide_rope_cos_sin_cache(
         cache: *mut f32,
@@ -424,6 +451,88 @@ extern "C" {
         slot_mapping: *mut i64,
         stream: HipStream,
     );
+
+    /// Metadata of a mixed step from request lengths: prefix sums, blocks handed out of `free_blocks` into the
+    /// tables, slots and positions.
+    pub fn build_step_metadata_device(
+        context_lens: *const u32,
+        query_lens: *const u32,
+        position_offsets: *const i32,
+        block_table: *mut i32,
+        max_blocks_per_seq: i64,
+        free_blocks: *const i32,
+        num_free_blocks: i64,
+        batch: i64,
+        block_size: i64,
+        num_tokens: i64,
+        num_axes: i64,
+        cu_seqlens_q: *mut u32,
+        cu_seqlens_k: *mut u32,
+        cu_new_blocks: *mut u32,
+        slot_mapping: *mut i64,
+        positions: *mut i32,
+        stream: HipStream,
+    );
+
+    /// Linear attention with a decay per head, one token per sequence; updates the fp32 states in place.
+    pub fn linear_attention_decode(
+        out: *mut c_void,
+        q: *const c_void,
+        k: *const c_void,
+        v: *const c_void,
+        q_row_stride: i64,
+        k_row_stride: i64,
+        v_row_stride: i64,
+        log_decay: *const f32,
+        state: *mut f32,
+        state_slots: *const i32,
+        num_slots: i64,
+        batch: i64,
+        num_heads: i64,
+        num_kv_heads: i64,
+        head_dim: i64,
+        scale: f32,
+        dtype: c_int,
+        stream: HipStream,
+    );
+
+    /// Linear attention with a decay per head over prompts, in chunks; `context_lens` may be null.
+    pub fn linear_attention_prefill(
+        out: *mut c_void,
+        q: *const c_void,
+        k: *const c_void,
+        v: *const c_void,
+        q_row_stride: i64,
+        k_row_stride: i64,
+        v_row_stride: i64,
+        log_decay: *const f32,
+        state: *mut f32,
+        state_slots: *const i32,
+        context_lens: *const u32,
+        cu_seqlens_q: *const u32,
+        num_slots: i64,
+        total_q: i64,
+        batch: i64,
+        num_heads: i64,
+        num_kv_heads: i64,
+        head_dim: i64,
+        max_seqlen_q: i64,
+        scale: f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        dtype: c_int,
+        stream: HipStream,
+    );
+
+    /// Workspace bytes of `linear_attention_prefill`; 0 where it uses none.
+    pub fn linear_attention_prefill_workspace_size(
+        total_q: i64,
+        batch: i64,
+        num_heads: i64,
+        num_kv_heads: i64,
+        head_dim: i64,
+        max_seqlen_q: i64,
+    ) -> usize;
 
     /// Allocation-free decode (graph capture, serving loops): partials in a 48 MiB static device
     /// array per GPU; larger shapes fail with OXIDE_ERR_SCRATCH_TOO_SMALL; overlapping calls on one GPU race.

@@ -50,6 +50,12 @@ inline int dtype_size(int dtype) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether na 16-bit elements from a and nb from b share one.
+inline bool overlap16(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + 2 * static_cast<uintptr_t>(nb) && y < x + 2 * static_cast<uintptr_t>(na);
+}
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 }  // namespace oxide

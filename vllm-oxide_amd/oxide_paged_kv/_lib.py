@@ -74,8 +74,19 @@ SIGNATURES = {
     "qk_norm_rope_and_cache": (None, [
         _p, _p, _p, _i64, _p, _p, ctypes.c_double, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
         ctypes.c_int, _p]),
+    "qk_norm_mrope_and_cache": (None, [
+        _p, _p, _p, _i64, _p, _p, ctypes.c_double, _p, _i64, _p, _i64, _p, ctypes.c_int, _p, _p, _i64, _p, _i64, _i64,
+        _i64, _i64, ctypes.c_int, _p]),
     "oxide_rope_cos_sin_cache": (ctypes.c_int, [_p, _i64, _i64, ctypes.c_float]),
     "build_decode_metadata_device": (None, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
+    "build_step_metadata_device": (None, [
+        _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "linear_attention_decode": (None, [
+        _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, _p]),
+    "linear_attention_prefill": (None, [
+        _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float,
+        _p, ctypes.c_size_t, ctypes.c_int, _p]),
+    "linear_attention_prefill_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "oxide_fill_normal": (ctypes.c_int, [_p, _i64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int, ctypes.c_int]),
     "oxide_last_error": (ctypes.c_int, []),
     "oxide_clear_error": (None, []),

@@ -16,11 +16,13 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <initializer_list>
 
 #include "oxide_paged_kv.h"
 
@@ -34,6 +36,11 @@ decltype(&varlen_prefill_attention_workspace) g_prefill_varlen = nullptr;
 decltype(&prefill_attention_workspace_size) g_prefill_ws = nullptr;
 decltype(&qk_norm_rope_and_cache) g_prologue = nullptr;
 decltype(&build_decode_metadata_device) g_metadata = nullptr;
+decltype(&qk_norm_mrope_and_cache) g_mrope = nullptr;
+decltype(&build_step_metadata_device) g_step_metadata = nullptr;
+decltype(&linear_attention_decode) g_linear_decode = nullptr;
+decltype(&linear_attention_prefill) g_linear_prefill = nullptr;
+decltype(&linear_attention_prefill_workspace_size) g_linear_ws = nullptr;
 decltype(&oxide_last_error) g_last_error = nullptr;
 
 // A plain torch tensor on the device, contiguous.
@@ -244,6 +251,222 @@ PyObject* metadata(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool same_device(const at::Tensor& t, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* o : others)
+    if (o && o->device() != t.device()) return false;
+  return true;
+}
+// A plain torch tensor [T, H, D] on the device whose rows are contiguous, any row stride.
+const at::Tensor* rows_tensor(PyObject* o, int64_t* stride) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.dim() != 3) return nullptr;
+  const int64_t T = t.size(0), H = t.size(1), D = t.size(2);
+  if ((D > 1 && t.stride(2) != 1) || (H > 1 && t.stride(1) != D)) return nullptr;
+  *stride = T > 1 ? t.stride(0) : H * D;
+  return &t;
+}
+
+// step_metadata(context_lens, query_lens, block_table, free_blocks, num_tokens, block_size,
+//               position_offsets, num_axes)
+//   -> (cu_seqlens_q, cu_seqlens_k, slot_mapping, positions, cu_new_blocks)
+PyObject* step_metadata(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !g_step_metadata) Py_RETURN_NONE;
+  const at::Tensor *ctx = device_tensor(a[0]), *query = device_tensor(a[1]), *table = device_tensor(a[2]),
+                   *free_list = nullptr, *offsets = nullptr;
+  int64_t rows = 0, page = 0, axes = 0;
+  if (!ctx || !query || !table || !optional_tensor(a[3], &free_list) || !as_int(a[4], &rows) || !as_int(a[5], &page) ||
+      !optional_tensor(a[6], &offsets) || (a[7] != Py_None && (!as_int(a[7], &axes) || axes < 1 || axes > 4)))
+    Py_RETURN_NONE;
+  if (!bits32(*ctx) || !bits32(*query) || ctx->dim() != 1 || query->sizes() != ctx->sizes() || table->dim() != 2 ||
+      table->size(0) != ctx->size(0) || table->scalar_type() != at::kInt || rows < 0 ||
+      (free_list && (free_list->scalar_type() != at::kInt || free_list->dim() != 1)) ||
+      (offsets && (offsets->scalar_type() != at::kInt || offsets->sizes() != ctx->sizes())) ||
+      !same_device(*ctx, {query, table, free_list, offsets}))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(ctx->device());
+  const int64_t B = ctx->size(0), width = table->size(1), free_n = free_list ? free_list->size(0) : 0;
+  const auto i32 = ctx->options().dtype(at::kInt);
+  at::Tensor cu_q = at::empty({B + 1}, i32), cu_k = at::empty({B + 1}, i32), cu_new = at::empty({B + 1}, i32);
+  at::Tensor slots = at::empty({rows}, i32.dtype(at::kLong));
+  at::Tensor pos = axes ? at::empty({axes, rows}, i32) : at::empty({rows}, i32);
+  void* s = stream_of(*ctx);
+  const uint32_t* pc = static_cast<const uint32_t*>(ctx->data_ptr());
+  const uint32_t* pq = static_cast<const uint32_t*>(query->data_ptr());
+  const int32_t *po = static_cast<const int32_t*>(data(offsets)), *pf = static_cast<const int32_t*>(data(free_list));
+  int32_t *pt = static_cast<int32_t*>(table->data_ptr()), *pp = static_cast<int32_t*>(pos.data_ptr());
+  uint32_t *pcq = static_cast<uint32_t*>(cu_q.data_ptr()), *pck = static_cast<uint32_t*>(cu_k.data_ptr()),
+           *pcn = static_cast<uint32_t*>(cu_new.data_ptr());
+  int64_t* ps = static_cast<int64_t*>(slots.data_ptr());
+  Py_BEGIN_ALLOW_THREADS;
+  g_step_metadata(pc, pq, po, pt, width, pf, free_n, B, page, rows, axes ? axes : 1, pcq, pck, pcn, ps, pp, s);
+  Py_END_ALLOW_THREADS;
+  if (g_last_error() != OXIDE_OK) Py_RETURN_FALSE;
+  PyObject* r = PyTuple_New(5);
+  if (!r) return nullptr;
+  at::Tensor* made[] = {&cu_q, &cu_k, &slots, &pos, &cu_new};
+  for (int i = 0; i < 5; ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(*made[i]));
+    if (!o) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i, o);
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// mrope(qkv, num_heads, num_kv_heads, q_norm_weight, k_norm_weight, eps, cos_sin_cache, positions,
+//       sections, key_cache, value_cache, slot_mapping, interleaved, q_out)
+PyObject* mrope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 14 || !g_mrope) Py_RETURN_NONE;
+  const at::Tensor *qkv = device_tensor(a[0]), *qw = nullptr, *kw = nullptr, *rope = device_tensor(a[6]),
+                   *pos = device_tensor(a[7]), *kc = nullptr, *vc = nullptr, *slots = nullptr, *out = nullptr;
+  int64_t Hq = 0, Hkv = 0;
+  double eps = 0;
+  if (!qkv || !rope || !pos || !as_int(a[1], &Hq) || !as_int(a[2], &Hkv) || !optional_tensor(a[3], &qw) ||
+      !optional_tensor(a[4], &kw) || !as_double(a[5], &eps) || !PyTuple_CheckExact(a[8]) ||
+      !optional_tensor(a[9], &kc) || !optional_tensor(a[10], &vc) || !optional_tensor(a[11], &slots) ||
+      !PyBool_Check(a[12]) || !optional_tensor(a[13], &out))
+    Py_RETURN_NONE;
+  const int64_t axes = PyTuple_GET_SIZE(a[8]);
+  int32_t sections[4] = {0, 0, 0, 0};
+  if (axes < 1 || axes > 4) Py_RETURN_NONE;
+  for (int64_t i = 0; i < axes; ++i) {
+    int64_t x = 0;
+    if (!as_int(PyTuple_GET_ITEM(a[8], i), &x) || x < 0 || x > INT32_MAX) Py_RETURN_NONE;
+    sections[i] = static_cast<int32_t>(x);
+  }
+  const int code = dtype_code(*qkv);
+  if (code < 0 || qkv->dim() != 2 || rope->dim() != 2 || rope->scalar_type() != at::kFloat || Hq < 1 || Hkv < 1 ||
+      Hq > 4096 || Hkv > 4096)
+    Py_RETURN_NONE;
+  const int64_t T = qkv->size(0), D = rope->size(1);
+  auto like_qkv = [&](const at::Tensor* t, at::IntArrayRef sizes) {
+    return t->sizes() == sizes && t->scalar_type() == qkv->scalar_type();
+  };
+  if (qkv->size(1) < (Hq + 2 * Hkv) * D || pos->scalar_type() != at::kInt || pos->sizes() != at::IntArrayRef({axes, T}) ||
+      (qw && !like_qkv(qw, {D})) || (kw && !like_qkv(kw, {D})) || (out && !like_qkv(out, {T, Hq, D})) ||
+      !same_device(*qkv, {qw, kw, rope, pos, kc, vc, slots, out}))
+    Py_RETURN_NONE;
+  if (slots ? !kc || !vc || kc->dim() != 4 || kc->sizes() != vc->sizes() || kc->size(2) != Hkv || kc->size(3) != D ||
+                  kc->scalar_type() != qkv->scalar_type() || vc->scalar_type() != qkv->scalar_type() ||
+                  slots->scalar_type() != at::kLong || slots->sizes() != at::IntArrayRef({T})
+            : kc || vc)
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(qkv->device());
+  at::Tensor o = out ? *out : at::empty({T, Hq, D}, qkv->options());
+  void* s = stream_of(*qkv);
+  void *po = o.data_ptr(), *px = qkv->data_ptr(), *pqw = data(qw), *pkw = data(kw), *pkc = data(kc), *pvc = data(vc);
+  const float* pr = static_cast<const float*>(rope->data_ptr());
+  const int32_t* pp = static_cast<const int32_t*>(pos->data_ptr());
+  const int64_t* ps = static_cast<const int64_t*>(data(slots));
+  const int64_t stride = qkv->size(1), max_position = rope->size(0), rows = slots ? kc->size(0) * kc->size(1) : 0;
+  const int dealt = a[12] == Py_True;
+  Py_BEGIN_ALLOW_THREADS;
+  g_mrope(po, nullptr, px, stride, pqw, pkw, eps, pr, max_position, pp, axes, sections, dealt, pkc, pvc, rows, ps, T,
+          Hq, Hkv, D, code, s);
+  Py_END_ALLOW_THREADS;
+  return result(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// The tensors of a linear attention call, checked as ops._check_linear does.
+struct Linear {
+  const at::Tensor *q, *k, *v, *decay, *state, *slots, *out;
+  int64_t sq, sk, sv, T, Hq, Hkv, D;
+  int code;
+};
+bool as_linear(PyObject* const* a, PyObject* out, Linear* x) {
+  x->q = rows_tensor(a[0], &x->sq);
+  x->k = rows_tensor(a[1], &x->sk);
+  x->v = rows_tensor(a[2], &x->sv);
+  x->decay = device_tensor(a[3]);
+  x->state = device_tensor(a[4]);
+  x->slots = device_tensor(a[5]);
+  if (!x->q || !x->k || !x->v || !x->decay || !x->state || !x->slots || !optional_tensor(out, &x->out)) return false;
+  x->T = x->q->size(0), x->Hq = x->q->size(1), x->D = x->q->size(2), x->Hkv = x->k->size(1);
+  x->code = dtype_code(*x->q);
+  return x->code >= 0 && x->k->size(0) == x->T && x->k->size(2) == x->D && x->v->sizes() == x->k->sizes() &&
+         x->Hkv > 0 && x->Hq % x->Hkv == 0 && x->k->scalar_type() == x->q->scalar_type() &&
+         x->v->scalar_type() == x->q->scalar_type() && x->decay->scalar_type() == at::kFloat &&
+         x->decay->sizes() == at::IntArrayRef({x->Hkv}) && x->state->scalar_type() == at::kFloat &&
+         x->state->dim() == 4 && x->state->size(1) == x->Hkv && x->state->size(2) == x->D &&
+         x->state->size(3) == x->D && x->slots->scalar_type() == at::kInt && x->slots->dim() == 1 &&
+         (!x->out || (x->out->sizes() == x->q->sizes() && x->out->scalar_type() == x->q->scalar_type())) &&
+         same_device(*x->q, {x->k, x->v, x->decay, x->state, x->slots, x->out});
+}
+
+// linear_decode(q, k, v, log_decay, state, state_slots, scale, out)
+PyObject* linear_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Linear x;
+  double scale = 0;
+  if (n != 8 || !g_linear_decode || !as_double(a[6], &scale) || !as_linear(a, a[7], &x) || x.slots->size(0) != x.T)
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(x.q->device());
+  at::Tensor o = x.out ? *x.out : at::empty({x.T, x.Hq, x.D}, x.q->options());
+  void* s = stream_of(*x.q);
+  void *po = o.data_ptr(), *pq = x.q->data_ptr(), *pk = x.k->data_ptr(), *pv = x.v->data_ptr();
+  const float* pd = static_cast<const float*>(x.decay->data_ptr());
+  float* pst = static_cast<float*>(x.state->data_ptr());
+  const int32_t* psl = static_cast<const int32_t*>(x.slots->data_ptr());
+  const int64_t num_slots = x.state->size(0);
+  Py_BEGIN_ALLOW_THREADS;
+  g_linear_decode(po, pq, pk, pv, x.sq, x.sk, x.sv, pd, pst, psl, num_slots, x.T, x.Hq, x.Hkv, x.D,
+                  static_cast<float>(scale), x.code, s);
+  Py_END_ALLOW_THREADS;
+  return result(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_prefill(q, k, v, log_decay, state, state_slots, cu_seqlens_q, max_seqlen_q, scale,
+//                context_lens, out, workspace)
+PyObject* linear_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Linear x;
+  double scale = 0;
+  int64_t max_q = 0;
+  const at::Tensor *cu = nullptr, *ctx = nullptr, *ws = nullptr;
+  if (n != 12 || !g_linear_prefill || !(cu = device_tensor(a[6])) || !as_int(a[7], &max_q) ||
+      !as_double(a[8], &scale) || !optional_tensor(a[9], &ctx) || !as_linear(a, a[10], &x) ||
+      !optional_tensor(a[11], &ws))
+    Py_RETURN_NONE;
+  const int64_t B = cu->numel() - 1;
+  if (!bits32(*cu) || cu->dim() != 1 || B < 0 || x.slots->size(0) != B ||
+      (ctx && (!bits32(*ctx) || ctx->sizes() != at::IntArrayRef({B}))) || !same_device(*x.q, {cu, ctx, ws}))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(x.q->device());
+  at::Tensor o = x.out ? *x.out : at::empty({x.T, x.Hq, x.D}, x.q->options());
+  at::Tensor w;
+  if (ws) {
+    w = *ws;
+  } else if (const size_t need = g_linear_ws(x.T, B, x.Hq, x.Hkv, x.D, max_q)) {
+    try {
+      w = bytes_like(*x.q, static_cast<int64_t>(need));
+    } catch (const c10::OutOfMemoryError&) {  // it works without one
+    }
+  }
+  void* s = stream_of(*x.q);
+  void *po = o.data_ptr(), *pq = x.q->data_ptr(), *pk = x.k->data_ptr(), *pv = x.v->data_ptr();
+  const float* pd = static_cast<const float*>(x.decay->data_ptr());
+  float* pst = static_cast<float*>(x.state->data_ptr());
+  const int32_t* psl = static_cast<const int32_t*>(x.slots->data_ptr());
+  const uint32_t *pcu = static_cast<const uint32_t*>(cu->data_ptr()), *pctx = static_cast<const uint32_t*>(data(ctx));
+  const int64_t num_slots = x.state->size(0);
+  void* pw = w.defined() ? w.data_ptr() : nullptr;
+  const size_t wbytes = w.defined() ? w.nbytes() : 0;
+  Py_BEGIN_ALLOW_THREADS;
+  g_linear_prefill(po, pq, pk, pv, x.sq, x.sk, x.sv, pd, pst, psl, pctx, pcu, num_slots, x.T, B, x.Hq, x.Hkv, x.D,
+                   max_q, static_cast<float>(scale), pw, wbytes, x.code, s);
+  Py_END_ALLOW_THREADS;
+  return result(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(name, address): the library's function of that name; names not used here are
 // accepted.
 PyObject* bind(PyObject*, PyObject* args) {
@@ -261,6 +484,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   OXIDE_BIND(g_prefill_ws, prefill_attention_workspace_size)
   OXIDE_BIND(g_prologue, qk_norm_rope_and_cache)
   OXIDE_BIND(g_metadata, build_decode_metadata_device)
+  OXIDE_BIND(g_mrope, qk_norm_mrope_and_cache)
+  OXIDE_BIND(g_step_metadata, build_step_metadata_device)
+  OXIDE_BIND(g_linear_decode, linear_attention_decode)
+  OXIDE_BIND(g_linear_prefill, linear_attention_prefill)
+  OXIDE_BIND(g_linear_ws, linear_attention_prefill_workspace_size)
   OXIDE_BIND(g_last_error, oxide_last_error)
 #undef OXIDE_BIND
   Py_RETURN_NONE;
@@ -272,6 +500,8 @@ PyMethodDef fast(const char* name) {
 }
 PyMethodDef kMethods[] = {fast<decode>("decode"),     fast<prefill>("prefill"),
                           fast<prologue>("prologue"), fast<metadata>("metadata"),
+                          fast<mrope>("mrope"),       fast<step_metadata>("step_metadata"),
+                          fast<linear_decode>("linear_decode"), fast<linear_prefill>("linear_prefill"),
                           {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
