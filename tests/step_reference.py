@@ -118,7 +118,7 @@ def assert_linear_close(got, want, size, dtype, longest, what):
     the state are each rounded once to the type on their way into the matrix products (half a
     step of the sum of absolute values that they are part of); fp32 sums over at most D + longest
     terms add 2^-24 of that sum each.  A state is held in fp32; the values that are added to it
-    go through the matrix products as two 16-bit parts, off by at most 2^-16.
+    go through the matrix products as 16-bit parts, together off by at most 2^-16.
     In the 2-norm, for inputs of independent signs, where errors add as the terms do: the three
     roundings together stay under twice a half step, the state's under 2^-19."""
     got = np.asarray(got, np.float64)

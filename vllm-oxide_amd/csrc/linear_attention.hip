@@ -34,9 +34,12 @@ struct LinearParams {
   const int32_t* slots;          // [batch]
   const uint32_t* context_lens;  // [batch] or null (prefill)
   const uint32_t* cu_q;          // [batch + 1] (prefill)
+  float* workspace;              // pieces' states (prefill)
   int64_t total_q;
   int64_t num_slots;
+  int64_t units;  // states of each kv head in the workspace
   int batch, num_heads, num_kv_heads, group, max_q;
+  int piece_tokens, pieces;  // tokens of a piece, pieces of the longest sequence
   float scale;
 };
 
@@ -127,72 +130,595 @@ __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) 
   }
 }
 
-// Prompts, token by token: a workgroup walks a sequence with 32 columns of the state in
-// registers.
-template <class Tag, int D>
-__global__ __launch_bounds__(kDecodeThreads) void linear_prefill_recurrent(LinearParams p) {
-  constexpr int kLanes = kDecodeCols / 4;
-  constexpr int kRows = kDecodeThreads / kLanes;
-  constexpr int N = D / kRows;
-  __shared__ float s_part[kDecodeThreads / 64][kDecodeCols];
-  const int slices = D / kDecodeCols;
-  const int slice = blockIdx.x % slices;
-  const int n = blockIdx.x / slices % p.num_kv_heads;
-  const int b = blockIdx.x / slices / p.num_kv_heads;
+// Prompts, 64 tokens at a time on the matrix cores.  With S the state before a chunk,
+// rows i, j of the chunk and n tokens in it:
+//   P_ij = (q_i . k_j) lambda^(i - j) for j <= i, else 0
+//   out_i = scale * (lambda^(i + 1) S^T q_i + sum_j P_ij v_j)
+//   S <- lambda^n S + sum_j k_j (lambda^(n - 1 - j) v_j)^T
+// A workgroup has a wave for each 32 value columns; a wave keeps its columns of S (all
+// key rows) in matrix-core accumulators from chunk to chunk.  Scores are shared: each
+// wave computes 16 query rows of P (two such strips at D = 64) and puts them into LDS.
+// A last chunk of fewer than 64 tokens is padded with zero rows in FRONT, so weights and
+// decays have their places in every chunk.
+//
+// Matrix-core layouts (cdna4_tile.hpp): the accumulator of K^T V has a value column in
+// each lane and key rows in registers, which is the operand layout of S^T if the eight
+// rows of a register run are those of an operand's k run: key columns are dealt to the
+// rows of a tile with bits 2 and 3 exchanged (deal), which the transposing LDS reads do
+// for nothing.  The same order for value columns hands a lane eight consecutive output
+// columns.
+//
+// What is rounded to 16 bits, and why: P and S are operands of 16-bit matrix products,
+// each rounded once (half a step of the type, as the output is); v times its weight
+// would be too, but lands in the fp32 state, so it goes through the products as a sum of
+// 16-bit values, three of bf16 or two of f16, with at least 22 bits.  f16 has the bits but not the
+// range: P's rows, a wave's part of S and of v are scaled by powers of two to about 2^14.
+//
+// v is used for every earlier row of a chunk as 0 * v, which is NaN for an infinity or
+// NaN: a chunk that holds one adds its products one by one instead.
+constexpr int kChunk = 64;
+
+template <int D>
+struct Tiles {
+  static constexpr int kWaves = D / 32;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kGranules = D / 8;       // 16-byte pieces of a row
+  static constexpr int kLoads = kChunk * kGranules / kThreads;  // granules of a tile a thread moves
+  static constexpr int kTileBytes = kChunk * kRowBytes;
+  static constexpr int kStrips = 4 / kWaves;  // 16-row strips of P a wave computes
+  static constexpr int kRegs = D * D / kThreads;  // state values of a lane
+  // Granule g of a row lies at g ^ turn(row): 16 rows' granules of one column, and four
+  // rows' of 32 columns, fall into different banks.  turn repeats every 16 rows, so an
+  // address is a lane's own offset, exclusive-or the granule, plus 16-row steps.
+  static __device__ __forceinline__ int turn(int row) {
+    if constexpr (D == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int row, int granule) {
+    return row * kRowBytes + ((granule ^ turn(row)) << 4);
+  }
+  static constexpr int kStep = 16 * kRowBytes;
+  // P's rows: 64 scores, 128 bytes.
+  static __device__ __forceinline__ int score_at(int row, int granule) {
+    return row * 128 + ((granule ^ ((row >> 1) & 7)) << 4);
+  }
+};
+
+// Column of a 32-column tile whose values row (or lane) m holds.
+__device__ __forceinline__ int deal(int m) { return (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// Offset of a lane's transposing reads of rows 8 (lane / 32) + 4 x + 0..3, columns dealt to
+// the lanes of a tile at column 0.
+template <int D>
+__device__ __forceinline__ int columns_at(int lane, int x) {
+  const int in_group = lane & 15, q = in_group & 3;
+  const int col = 16 * ((lane >> 4) & 1) + 8 * (q & 1) + 4 * (q >> 1);
+  return Tiles<D>::at(8 * (lane >> 5) + 4 * x + (in_group >> 2), col >> 3) + (col & 4) * 2;
+}
+// Operand of tokens 16 kb + 8 (lane / 32) + 0..7, column 32 t + deal(lane % 32).
+template <int D>
+__device__ __forceinline__ uint4 columns_operand(const char* tile, int at0, int at1, int kb, int t) {
+  const uint2 a = lds_read_tr16(tile + (at0 ^ (t << 6)) + kb * Tiles<D>::kStep);
+  const uint2 b = lds_read_tr16(tile + (at1 ^ (t << 6)) + kb * Tiles<D>::kStep);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// The compiler's scheduler moves nothing across: left alone it reads operands far ahead of
+// their products, into more registers than there are.
+__device__ __forceinline__ void fence_schedule() { __builtin_amdgcn_sched_barrier(0); }
+
+// Keeps a lane's offset one register: what is computed from it is not kept from chunk to
+// chunk in registers of its own.
+__device__ __forceinline__ int fresh_copy(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ uint4 lds_read16(const char* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// Whether one of eight packed values is an infinity or NaN.
+template <class Tag>
+__device__ __forceinline__ bool any_wild(uint4 v) {
+  constexpr bool bf16 = std::is_same<Tag, Bf16Tag>::value;
+  constexpr uint32_t mask = bf16 ? 0x7f807f80u : 0x7c007c00u, one = bf16 ? 0x00800080u : 0x04000400u;
+  return ((((v.x & mask) + one) | ((v.y & mask) + one) | ((v.z & mask) + one) | ((v.w & mask) + one)) & 0x80008000u) != 0;
+}
+
+template <class Tag>
+__device__ __forceinline__ void unpack8(uint4 v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = to_f32(Tag{}, static_cast<uint16_t>(w[e]));
+    x[2 * e + 1] = to_f32(Tag{}, static_cast<uint16_t>(w[e] >> 16));
+  }
+}
+template <class Tag>
+__device__ __forceinline__ uint4 pack8(const float* x) {
+  return make_uint4(pack2_cvt(Tag{}, x[0], x[1]), pack2_cvt(Tag{}, x[2], x[3]), pack2_cvt(Tag{}, x[4], x[5]),
+                    pack2_cvt(Tag{}, x[6], x[7]));
+}
+
+// 2^e with |x| 2^-e in [2^14, 2^15), e cut to +-40: beyond that 2^-65 of an f16 product's
+// range is lost, or an f16 overflow is honest.
+struct Pow2 {
+  float up, down;  // 2^e, 2^-e
+};
+__device__ __forceinline__ Pow2 scale_for_f16(float x) {
+  const int e = min(max(static_cast<int>((__float_as_uint(x) >> 23) & 255) - 127 - 14, -40), 40);
+  return Pow2{__uint_as_float(static_cast<uint32_t>(127 + e) << 23), __uint_as_float(static_cast<uint32_t>(127 - e) << 23)};
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_over_lane_groups(x);
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
+  return x;
+}
+
+// Values that are the same in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(uniform(__float_as_int(x))); }
+__device__ __forceinline__ Decay uniform(Decay d) { return Decay{uniform(d.hi), uniform(d.lo)}; }
+
+// A sequence's rows: at most max_q, and none past the last there is.
+struct Rows {
+  int begin, end;
+};
+__device__ __forceinline__ Rows rows_of(const LinearParams& p, int b) {
+  const int64_t begin = min(static_cast<int64_t>(p.cu_q[b]), p.total_q);
+  const int64_t end = min(min(static_cast<int64_t>(p.cu_q[b + 1]), p.total_q), begin + p.max_q);
+  return Rows{static_cast<int>(begin), static_cast<int>(end)};
+}
+
+// What a launch does with its pieces of sequences.
+enum Mode {
+  kWhole,   // a sequence from its slot's state to its end
+  kSums,    // a piece's own sum, from a zero state, into the workspace; not the last piece's
+  kPieces,  // a piece's outputs, from its begin's state in the workspace
+};
+
+template <class Tag, int D, int MODE>
+__global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(LinearParams p) {
+  using T = Tiles<D>;
+  constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
+  constexpr int kMt = D / 32;  // tiles of 32 key rows
+  __shared__ char s_k[T::kTileBytes] __attribute__((aligned(16)));
+  __shared__ char s_v[T::kTileBytes] __attribute__((aligned(16)));
+  __shared__ char s_q[MODE == kSums ? 16 : T::kTileBytes] __attribute__((aligned(16)));
+  __shared__ char s_p[MODE == kSums ? 16 : kChunk * 128] __attribute__((aligned(16)));
+  __shared__ float s_power[kChunk + 1];                            // lambda^m
+  __shared__ float s_weight[kChunk] __attribute__((aligned(16)));  // lambda^(63 - j)
+  __shared__ float s_up[kChunk];                                   // f16: 2^e of P's rows
+  __shared__ int s_wild;  // 1 + the last chunk that held an infinity or NaN in v
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), half = lane >> 5;
+  const int n = blockIdx.x % p.num_kv_heads;
+  const int piece = MODE == kWhole ? 0 : blockIdx.x / p.num_kv_heads % p.pieces;
+  const int b = blockIdx.x / p.num_kv_heads / (MODE == kWhole ? 1 : p.pieces);
   const int64_t slot = p.slots[b];
   if (slot < 0 || slot >= p.num_slots) return;
-  const int64_t begin = p.cu_q[b];
-  const int64_t end = min(min(static_cast<int64_t>(p.cu_q[b + 1]), p.total_q), begin + p.max_q);
-  if (end <= begin) return;
-  const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
-  const int col = slice * kDecodeCols + lane * 4;
-  float* state = p.state + (slot * p.num_kv_heads + n) * D * D + col;
-  const bool fresh = p.context_lens && p.context_lens[b] == 0;
-  floatx4 s[N];
+  const Rows rows = rows_of(p, b);
+  const int begin = uniform(rows.begin), end = uniform(rows.end);
+  const int t0 = begin + (MODE == kWhole ? 0 : min(end - begin, piece * p.piece_tokens));
+  if (t0 >= end) return;
+  const int t1 = MODE == kWhole ? end : t0 + min(end - t0, p.piece_tokens);
+  const bool last = t1 == end;
+  if (MODE == kSums && last) return;
+  // The piece's state in the workspace: every sequence has floor(begin / piece_tokens) ...
+  // on for its own.
+  const int64_t unit = MODE == kWhole ? 0 : begin / p.piece_tokens + piece - (MODE == kPieces ? 1 : 0);
+  if (MODE == kSums && unit >= p.units) return;
+  float* const ws = p.workspace + (unit * p.num_kv_heads + n) * D * D + tid * 4;
+  float* const state = p.state + (slot * p.num_kv_heads + n) * D * D + 32 * wave + deal(lane & 31);
+
+  const float ld = p.log_decay[n];
+  const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
+  for (int m = tid; m <= kChunk; m += T::kThreads) {
+    const float x = decay_power(ld, m).hi;
+    s_power[m] = x;
+    if (m < kChunk) s_weight[kChunk - 1 - m] = x;
+  }
+  if (tid == 0) s_wild = 0;
+  const Decay over_chunk = uniform(decay_power(ld, kChunk));
+  const Decay over_last = uniform(decay_power(ld, t1 - t0 - (chunks - 1) * kChunk));
+
+  // Lane's state values: register 8 a + i of tile mt is key row 32 mt + 16 a + 8 half + i.
+  floatx16 S[kMt];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    s[i] = fresh ? floatx4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const floatx4*>(state + (i * kRows + row) * D);
-  const Decay decay = decay_power(p.log_decay[n], 1);
-  for (int64_t t = begin; t < end; ++t) {
-    const uint16_t* k = p.k + t * p.k_stride + n * D;
-    const uint16_t* v = p.v + t * p.v_stride + n * D + col;
-    float vv[4];
+  for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) vv[e] = to_f32(Tag{}, v[e]);
+    for (int r = 0; r < 16; ++r) S[mt][r] = 0.f;
+  if (MODE == kPieces && piece > 0) {
+    if (unit < p.units) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float kk = to_f32(Tag{}, k[i * kRows + row]);
+      for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kk, vv[e], decay * s[i][e]);
+        for (int r = 0; r < 16; r += 4) {
+          const floatx4 x = *reinterpret_cast<const floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[mt][r + e] = x[e];
+        }
     }
-    for (int g = 0; g < p.group; ++g) {
-      const uint16_t* q = p.q + t * p.q_stride + (n * p.group + g) * D;
-      floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  } else if (MODE != kSums && !(p.context_lens && p.context_lens[b] == 0)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float qq = to_f32(Tag{}, q[i * kRows + row]);
+    for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = fmaf(qq, s[i][e], sum[e]);
-      }
+      for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
+  }
+
+  // Decays of the wave's scores: query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
+  float fade[T::kStrips][4][4];
+  if constexpr (MODE != kSums) {
+    __syncthreads();
 #pragma unroll
-      for (int m = kLanes; m < 64; m <<= 1)
+    for (int x = 0; x < T::kStrips; ++x) {
+      const int strip = x == 0 ? wave : 3 - wave;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], m);
-      __syncthreads();
-      if ((threadIdx.x & 63) < kLanes) *reinterpret_cast<floatx4*>(&s_part[threadIdx.x >> 6][lane * 4]) = sum;
-      __syncthreads();
-      if (threadIdx.x < kDecodeCols) {
-        float o = 0.f;
+      for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int w = 0; w < kDecodeThreads / 64; ++w) o += s_part[w][threadIdx.x];
-        p.out[(t * p.num_heads + n * p.group + g) * D + slice * kDecodeCols + threadIdx.x] =
-            pack1(Tag{}, o * p.scale);
-      }
+        for (int r = 0; r < 4; ++r)
+          fade[x][kt][r] = s_power[max(16 * strip + (lane & 15) - (16 * kt + 4 * (lane >> 4) + r), 0)];
     }
   }
+
+  // A thread moves granule tid % kGranules of rows tid / kGranules + 16 i of a tile.
+  const int tile_row = tid / T::kGranules, tile_at = T::at(tile_row, tid % T::kGranules);
+  auto lane_bytes = [&](int64_t stride) {
+    return static_cast<uint32_t>(tile_row) * static_cast<uint32_t>(stride * 2) + tid % T::kGranules * 16;
+  };
+  const uint32_t q_lane = lane_bytes(p.q_stride), k_lane = lane_bytes(p.k_stride), v_lane = lane_bytes(p.v_stride);
+  // Rows from `first` (of the chunk) on hold tokens; in place of those before, row `first`
+  // is read, and zeros are stored for k and v.
+  struct Granules {
+    uint4 r[T::kLoads];
+  };
+  auto load_tile = [&](const uint16_t* base, int64_t stride, uint32_t at, int64_t row0, int first) {
+    const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
+    Granules x;
+    if (first > 0) at = tid % T::kGranules * 16;
 #pragma unroll
-  for (int i = 0; i < N; ++i) *reinterpret_cast<floatx4*>(state + (i * kRows + row) * D) = s[i];
+    for (int i = 0; i < T::kLoads; ++i) {
+      uint32_t skip = 0;
+      if (first > 0) skip = static_cast<uint32_t>(max(16 * i + tile_row, first)) * static_cast<uint32_t>(stride * 2);
+      x.r[i] = *reinterpret_cast<const uint4*>(rows + (first > 0 ? 0 : i * 32 * stride) + (at + skip));
+    }
+    return x;
+  };
+  auto store_tile = [&](char* tile, const Granules& x) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) *reinterpret_cast<uint4*>(tile + tile_at + i * T::kStep) = x.r[i];
+  };
+  auto without_padding = [&](Granules x, int first) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i)
+      if (16 * i + tile_row < first) x.r[i] = make_uint4(0, 0, 0, 0);
+    return x;
+  };
+
+  const uint16_t* const qn = p.q + static_cast<int64_t>(n) * p.group * D;
+  const uint16_t* const kn = p.k + static_cast<int64_t>(n) * D;
+  const uint16_t* const vn = p.v + static_cast<int64_t>(n) * D;
+  // Chunk c is rows row0(c) + 0..63 of which the first first(c) are padding.
+  auto first_of = [&](int c) { return c + 1 < chunks ? 0 : chunks * kChunk - (t1 - t0); };
+  auto row0_of = [&](int c) { return static_cast<int64_t>(t0) + c * kChunk - first_of(c); };
+
+  // Offsets of the lane's operands in the tiles.
+  const int rows16 = T::at(lane & 15, lane >> 4), rows32 = T::at(lane & 31, half);
+  const int cols0 = columns_at<D>(lane, 0), cols1 = columns_at<D>(lane, 1);
+  const int scores16 = T::score_at(lane & 15, half) + ((lane >> 4) & 1) * 8, scores32 = T::score_at(lane & 31, half);
+  const uint32_t out_lane = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(p.num_heads * D * 2) +
+                            (32 * wave + 8 * half) * 2;
+
+  Granules rk = load_tile(kn, p.k_stride, k_lane, row0_of(0), first_of(0));
+  Granules rv = load_tile(vn, p.v_stride, v_lane, row0_of(0), first_of(0));
+  Granules rq{};
+  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, q_lane, row0_of(0), first_of(0));
+
+  for (int c = 0; c < chunks; ++c) {
+    const int first = first_of(c);
+    const int64_t row0 = row0_of(c);
+    if (first > 0) {
+      rk = without_padding(rk, first);
+      rv = without_padding(rv, first);
+    }
+    store_tile(s_k, rk);
+    store_tile(s_v, rv);
+    if constexpr (MODE != kSums) {
+      store_tile(s_q, rq);
+      bool wild = false;
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) wild |= any_wild<Tag>(rv.r[i]);
+      if (wild) s_wild = c + 1;
+    }
+    __syncthreads();
+    if (c + 1 < chunks) {
+      rk = load_tile(kn, p.k_stride, k_lane, row0_of(c + 1), first_of(c + 1));
+      rv = load_tile(vn, p.v_stride, v_lane, row0_of(c + 1), first_of(c + 1));
+    }
+    if constexpr (MODE != kSums) {
+      Pow2 s_scale{1.f, 1.f};
+      if constexpr (kF16) {
+        float m = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(S[mt][r]));
+        s_scale = scale_for_f16(wave_max(m));
+      }
+
+      for (int g = 0; g < p.group; ++g) {
+        if (g > 0) {
+          store_tile(s_q, rq);
+          __syncthreads();
+        }
+        const bool same = g + 1 < p.group;  // the next tile of queries is this chunk's
+        if (same || c + 1 < chunks)
+          rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, q_lane, same ? row0 : row0_of(c + 1),
+                         same ? first : first_of(c + 1));
+
+        // Scores: K Q^T tiles, a query in each lane and four keys in its registers.
+        const int r16 = fresh_copy(rows16), p16 = fresh_copy(scores16);
+#pragma unroll
+        for (int x = 0; x < T::kStrips; ++x) {
+          const int strip = x == 0 ? wave : 3 - wave;
+          uint4 qb[D / 32];
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk) qb[kk] = lds_read16(s_q + (r16 ^ (kk << 6)) + strip * T::kStep);
+          floatx4 score[4];
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) {
+            score[kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (kt <= strip) {
+#pragma unroll
+              for (int kk = 0; kk < D / 32; ++kk)
+                score[kt] = mfma16x16x32(Tag{}, lds_read16(s_k + (r16 ^ (kk << 6)) + kt * T::kStep), qb[kk], score[kt]);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const bool seen = kt < strip || 4 * (lane >> 4) + r <= (lane & 15);
+                score[kt][r] = seen ? score[kt][r] * fade[x][kt][r] : 0.f;
+              }
+            }
+          }
+          fence_schedule();
+          Pow2 p_scale{1.f, 1.f};
+          if constexpr (kF16) {
+            float m = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(score[kt][r]));
+            p_scale = scale_for_f16(max_over_lane_groups(m));
+            if (lane < 16) s_up[16 * strip + lane] = p_scale.up;
+          }
+          // Tiles of keys behind the strip are read only where they share a block of 32.
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) {
+            if (kt > (strip | 1)) continue;
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = kF16 ? score[kt][r] * p_scale.down : score[kt][r];
+            *reinterpret_cast<uint2*>(s_p + (p16 ^ (kt << 5)) + strip * 16 * 128) =
+                make_uint2(pack2_cvt(Tag{}, y[0], y[1]), pack2_cvt(Tag{}, y[2], y[3]));
+          }
+        }
+        __syncthreads();
+
+        fence_schedule();
+        // Outputs, transposed: a query (of both halves of the chunk) in each lane, value
+        // columns in its registers.
+        const int r32 = fresh_copy(rows32), p32 = fresh_copy(scores32);
+        floatx16 acc[2];
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[it][r] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = kF16 ? S[mt][8 * a + i] * s_scale.down : S[mt][8 * a + i];
+            const uint4 s16 = pack8<Tag>(x);
+#pragma unroll
+            for (int it = 0; it < 2; ++it)
+              acc[it] = mfma32x32x16(Tag{}, s16, lds_read16(s_q + (r32 ^ ((4 * mt + 2 * a) << 4)) + it * 2 * T::kStep),
+                                     acc[it]);
+            fence_schedule();
+          }
+        Pow2 p_scale[2] = {{1.f, 1.f}, {1.f, 1.f}};
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int query = 32 * it + (lane & 31);
+          float carry = s_power[max(query + 1 - first, 0)];
+          if constexpr (kF16) {
+            p_scale[it].up = s_up[query];
+            p_scale[it].down = __uint_as_float(0x7f000000u - __float_as_uint(p_scale[it].up));  // 1 / 2^e
+            carry *= s_scale.up * p_scale[it].down;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[it][r] *= carry;
+        }
+        if (s_wild != c + 1) {
+          const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) {
+            const uint4 v = columns_operand<D>(s_v, v0, v1, kb, wave);
+#pragma unroll
+            for (int it = kb / 2; it < 2; ++it)
+              acc[it] = mfma32x32x16(Tag{}, v, lds_read16(s_p + (p32 ^ (kb << 5)) + it * 32 * 128), acc[it]);
+            fence_schedule();
+          }
+        } else {
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            const int query = 32 * it + (lane & 31);
+            for (int j = 0; j < 32 * it + 32; ++j) {
+              const float pj = to_f32(
+                  Tag{}, *reinterpret_cast<const uint16_t*>(s_p + T::score_at(query, j >> 3) + (j & 7) * 2));
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                float x[8];
+                unpack8<Tag>(lds_read16(s_v + T::at(j, 4 * wave + 2 * a + half)), x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (j <= query) acc[it][8 * a + i] = fmaf(pj, x[i], acc[it][8 * a + i]);
+              }
+            }
+          }
+        }
+        char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int query = 32 * it + (lane & 31);
+          if (query >= first) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              float x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                x[i] = (kF16 ? acc[it][8 * a + i] * p_scale[it].up : acc[it][8 * a + i]) * p.scale;
+              *reinterpret_cast<uint4*>(out + it * 32 * static_cast<int64_t>(p.num_heads * D * 2) + out_lane + 32 * a) =
+                  pack8<Tag>(x);
+            }
+          }
+        }
+        if (g + 1 < p.group) __syncthreads();
+      }
+    }
+
+    fence_schedule();
+    if (MODE == kSums || c + 1 < chunks || last) {
+      Decay fall = c + 1 < chunks ? over_chunk : over_last;
+      Pow2 v_scale{1.f, 1.f};
+      const int k0 = fresh_copy(cols0), k1 = fresh_copy(cols1);
+      if constexpr (kF16) {
+        float m = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          float x[8];
+          unpack8<Tag>(columns_operand<D>(s_v, k0, k1, kb, wave), x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+        }
+        v_scale = scale_for_f16(wave_max(m));
+        fall.hi *= v_scale.down;
+        fall.lo *= v_scale.down;
+      }
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[mt][r] = fall * S[mt][r];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        float x[8], y[8];
+        unpack8<Tag>(columns_operand<D>(s_v, k0, k1, kb, wave), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] *= s_weight[16 * kb + 8 * half + i];
+          if constexpr (kF16) x[i] *= v_scale.down;
+        }
+        constexpr int kTerms = kF16 ? 2 : 3;
+        uint4 term[kTerms];
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) {
+          term[t] = pack8<Tag>(x);
+          unpack8<Tag>(term[t], y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] -= y[i];
+        }
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          const uint4 k = columns_operand<D>(s_k, k0, k1, kb, mt);
+#pragma unroll
+          for (int t = 0; t < kTerms; ++t) S[mt] = mfma32x32x16(Tag{}, k, term[t], S[mt]);
+        }
+        fence_schedule();
+      }
+      if constexpr (kF16) {
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[mt][r] *= v_scale.up;
+      }
+    }
+    __syncthreads();
+  }
+
+  if (MODE == kSums) {
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4) =
+            floatx4{S[mt][r], S[mt][r + 1], S[mt][r + 2], S[mt][r + 3]};
+  } else if (last) {
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D] = S[mt][r];
+  }
 }
+
+// The pieces' sums become the states at the next pieces' begins, in place:
+//   start(0) = the slot's state or zero, start(i + 1) = lambda^piece_tokens start(i) + sum(i).
+// A thread carries four values of a state through its sequence's pieces.
+template <int D>
+__global__ __launch_bounds__(256) void linear_prefill_join(LinearParams p) {
+  using T = Tiles<D>;
+  constexpr int kQuads = D * D / 4;
+  const int blocks = kQuads / 256;
+  const int quad = blockIdx.x % blocks * 256 + threadIdx.x;
+  const int n = blockIdx.x / blocks % p.num_kv_heads;
+  const int b = blockIdx.x / blocks / p.num_kv_heads;
+  const int64_t slot = p.slots[b];
+  if (slot < 0 || slot >= p.num_slots) return;
+  const Rows rows = rows_of(p, b);
+  const int begin = rows.begin;
+  const int sums = rows.end > begin ? (rows.end - begin - 1) / p.piece_tokens : 0;  // all pieces but the last
+  if (sums == 0) return;
+  // Where the workspace's quad lies in the state (as linear_prefill_chunks keeps it).
+  const int tid = quad % T::kThreads, part = quad / T::kThreads, lane = tid & 63;
+  const int row = 32 * (part / 4) + 16 * (part % 4 / 2) + 8 * (lane >> 5) + 4 * (part % 2);
+  const int col = 32 * (tid >> 6) + deal(lane & 31);
+  floatx4 s = {0.f, 0.f, 0.f, 0.f};
+  if (!(p.context_lens && p.context_lens[b] == 0)) {
+    const float* state = p.state + (slot * p.num_kv_heads + n) * D * D + row * D + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = state[e * D];
+  }
+  const Decay fall = decay_power(p.log_decay[n], p.piece_tokens);
+  const int64_t first = begin / p.piece_tokens;
+  for (int i = 0; i < sums && first + i < p.units; ++i) {
+    float* ws = p.workspace + ((first + i) * p.num_kv_heads + n) * D * D + quad * 4;
+    const floatx4 add = *reinterpret_cast<const floatx4*>(ws);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = fall * s[e] + add[e];
+    *reinterpret_cast<floatx4*>(ws) = s;
+  }
+}
+
+// Tokens of a piece, 0 where sequences are walked whole.
+struct Plan {
+  int64_t piece_tokens, units;
+};
+Plan plan_prefill(int64_t total_q, int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                  int64_t max_seqlen_q) {
+  const Plan whole{0, 0};
+  if (total_q <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128) || max_seqlen_q <= 0)
+    return whole;
+  const int64_t wanted = 2 * oxide::device_cu_count();  // workgroups
+  if (batch * num_kv_heads >= wanted) return whole;
+  int64_t piece = (total_q * num_kv_heads + wanted - 1) / wanted;
+  piece = (piece + kChunk - 1) / kChunk * kChunk;
+  if (piece < 256) piece = 256;
+  if (max_seqlen_q <= 2 * piece) return whole;
+  return Plan{piece, total_q / piece};
+}
+
+constexpr int64_t kMaxStride = 1 << 26;  // elements: 16 rows' offsets in bytes fit 32 bits
 
 // Argument checks of both entries; OXIDE_OK, or the error to record.
 int check_linear(const LinearParams& p, int64_t rows, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
@@ -202,7 +728,8 @@ int check_linear(const LinearParams& p, int64_t rows, int64_t batch, int64_t num
   if (batch < 0 || rows < 0 || batch > 65535 || rows > INT32_MAX || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads > 4096 || num_heads % num_kv_heads != 0 || p.num_slots < 0 || p.q_stride < num_heads * head_dim ||
       p.k_stride < num_kv_heads * head_dim || p.v_stride < num_kv_heads * head_dim || p.q_stride % 8 != 0 ||
-      p.k_stride % 8 != 0 || p.v_stride % 8 != 0)
+      p.k_stride % 8 != 0 || p.v_stride % 8 != 0 || p.q_stride > kMaxStride || p.k_stride > kMaxStride ||
+      p.v_stride > kMaxStride)
     return OXIDE_ERR_INVALID_ARGUMENT;
   if (batch == 0 || rows == 0) return OXIDE_OK;
   const void* ptrs[] = {p.out, p.q, p.k, p.v, p.state};
@@ -285,7 +812,8 @@ extern "C" void linear_attention_decode(void* out, const void* q, const void* k,
 extern "C" size_t linear_attention_prefill_workspace_size(int64_t total_q, int64_t batch, int64_t num_heads,
                                                           int64_t num_kv_heads, int64_t head_dim,
                                                           int64_t max_seqlen_q) {
-  return 0;
+  const Plan plan = plan_prefill(total_q, batch, num_heads, num_kv_heads, head_dim, max_seqlen_q);
+  return static_cast<size_t>(plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
 }
 
 extern "C" void linear_attention_prefill(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,
@@ -311,12 +839,27 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
   p.cu_q = cu_seqlens_q;
   p.total_q = total_q;
   p.max_q = static_cast<int>(max_seqlen_q < total_q ? max_seqlen_q : total_q);
+  const Plan plan = plan_prefill(total_q, batch, num_heads, num_kv_heads, head_dim, max_seqlen_q);
+  const size_t need = static_cast<size_t>(plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
+  const bool cut = plan.piece_tokens > 0 && workspace && oxide::aligned16(workspace) && workspace_bytes >= need;
+  hipStream_t s = oxide::as_stream(stream);
   dispatch(dtype, head_dim, [&](auto tag, auto d) {
     using Tag = decltype(tag);
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((linear_prefill_recurrent<Tag, D>),
-                       dim3(static_cast<unsigned>(batch * num_kv_heads * (D / kDecodeCols))), dim3(kDecodeThreads), 0,
-                       oxide::as_stream(stream), p);
+    const dim3 threads(Tiles<D>::kThreads);
+    const unsigned heads = static_cast<unsigned>(batch * num_kv_heads);
+    if (!cut) {
+      hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kWhole>), dim3(heads), threads, 0, s, p);
+      return;
+    }
+    p.workspace = static_cast<float*>(workspace);
+    p.units = plan.units;
+    p.piece_tokens = static_cast<int>(plan.piece_tokens);
+    p.pieces = static_cast<int>((p.max_q + plan.piece_tokens - 1) / plan.piece_tokens);
+    const dim3 grid(heads * static_cast<unsigned>(p.pieces));
+    hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kSums>), grid, threads, 0, s, p);
+    hipLaunchKernelGGL((linear_prefill_join<D>), dim3(heads * (D * D / 4 / 256)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), grid, threads, 0, s, p);
   });
   oxide::check_launch();
 }
