@@ -58,6 +58,22 @@ __device__ __forceinline__ Decay decay_power(float log_decay, int n) {
   return Decay{hi, __builtin_isinf(hi) ? 0.f : static_cast<float>(e - static_cast<double>(hi))};
 }
 
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+// Powers of lambda one after the other, each a single fp32 factor: what its rounding leaves
+// out is put into the next one, so the product of any run of them is off by a few 2^-25.
+struct DecaySteps {
+  float off = 0.f;  // relative, of the factors so far
+  __device__ __forceinline__ float next(Decay d) {
+    const bool plain = d.hi > 0.f && !__builtin_isinf(d.hi);
+    const float add = plain ? fmaf(d.hi, off, d.lo) : d.lo;
+    const float f = d.hi + add;
+    off = plain ? (add - (f - d.hi)) * __builtin_amdgcn_rcpf(d.hi) : 0.f;
+    return f;
+  }
+};
+
 constexpr int kDecodeThreads = 256;
 constexpr int kDecodeCols = 32;  // state columns of a workgroup
 
@@ -208,6 +224,18 @@ __device__ __forceinline__ uint4 columns_operand(const char* tile, int at0, int 
 // their products, into more registers than there are.
 __device__ __forceinline__ void fence_schedule() { __builtin_amdgcn_sched_barrier(0); }
 
+// Asks for READS LDS reads first, then PRODUCTS matrix products with VALU others between
+// each two: a product keeps the matrix cores busy for as long as eight of those take.
+template <int READS, int PRODUCTS, int VALU>
+__device__ __forceinline__ void interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+
 // Keeps a lane's offset one register: what is computed from it is not kept from chunk to
 // chunk in registers of its own.
 __device__ __forceinline__ int fresh_copy(int x) {
@@ -217,12 +245,24 @@ __device__ __forceinline__ int fresh_copy(int x) {
 
 __device__ __forceinline__ uint4 lds_read16(const char* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// Whether one of eight packed values is an infinity or NaN.
-template <class Tag>
-__device__ __forceinline__ bool any_wild(uint4 v) {
-  constexpr bool bf16 = std::is_same<Tag, Bf16Tag>::value;
-  constexpr uint32_t mask = bf16 ? 0x7f807f80u : 0x7c007c00u, one = bf16 ? 0x00800080u : 0x04000400u;
-  return ((((v.x & mask) + one) | ((v.y & mask) + one) | ((v.z & mask) + one) | ((v.w & mask) + one)) & 0x80008000u) != 0;
+// acc + 0 * (each of eight packed bf16 values): NaN once one of them is an infinity or NaN.
+__device__ __forceinline__ float add_zeros(uint4 v, float acc) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_in_t, w[e]), __builtin_bit_cast(bf16x2_in_t, 0u), acc,
+                                          false);
+  return acc;
+}
+// The larger of `most` and the magnitudes of eight packed f16 values, as bit patterns (which
+// are ordered as the magnitudes are), low and high ones apart; 0x7c00 on: infinity, NaN.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2_t max_bits(uint4 v, u16x2_t most) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[e] & 0x7fff7fffu));
+  return most;
 }
 
 template <class Tag>
@@ -249,11 +289,17 @@ __device__ __forceinline__ Pow2 scale_for_f16(float x) {
   const int e = min(max(static_cast<int>((__float_as_uint(x) >> 23) & 255) - 127 - 14, -40), 40);
   return Pow2{__uint_as_float(static_cast<uint32_t>(127 + e) << 23), __uint_as_float(static_cast<uint32_t>(127 - e) << 23)};
 }
+// Largest of a wave's values, in every lane: over rows of 16 lanes by rotations within them
+// (an LDS shuffle would be a round trip each), then over the four rows.
 __device__ __forceinline__ float wave_max(float x) {
-  x = max_over_lane_groups(x);
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
+#define OXIDE_ROTATED_MAX(N) \
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + N, 0xf, 0xf, true)))
+  OXIDE_ROTATED_MAX(1);
+  OXIDE_ROTATED_MAX(2);
+  OXIDE_ROTATED_MAX(4);
+  OXIDE_ROTATED_MAX(8);
+#undef OXIDE_ROTATED_MAX
+  return max_over_lane_groups(x);
 }
 
 // Values that are the same in every lane, in scalar registers.
@@ -290,7 +336,9 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   __shared__ float s_power[kChunk + 1];                            // lambda^m
   __shared__ float s_weight[kChunk] __attribute__((aligned(16)));  // lambda^(63 - j)
   __shared__ float s_up[kChunk];                                   // f16: 2^e of P's rows
-  __shared__ int s_wild;  // 1 + the last chunk that held an infinity or NaN in v
+  // Of even and odd chunks: bf16, whether v holds an infinity or NaN; f16, its largest
+  // magnitude's bits (0x7c00 on: one of those).
+  __shared__ int s_most[2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), half = lane >> 5;
   const int n = blockIdx.x % p.num_kv_heads;
@@ -319,7 +367,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     s_power[m] = x;
     if (m < kChunk) s_weight[kChunk - 1 - m] = x;
   }
-  if (tid == 0) s_wild = 0;
+  if (tid < 2) s_most[tid] = 0;
   const Decay over_chunk = uniform(decay_power(ld, kChunk));
   const Decay over_last = uniform(decay_power(ld, t1 - t0 - (chunks - 1) * kChunk));
 
@@ -347,18 +395,22 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
   }
 
-  // Decays of the wave's scores: query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
+  // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
+  // Strips have one to four tiles of keys: of two workgroups on a compute unit (neighbours in
+  // the grid 8 or 256 apart) one deals them out in reverse, so that its SIMDs get even work.
+  const int strip0 = T::kStrips == 1 && ((blockIdx.x >> 3 ^ blockIdx.x >> 8) & 1) ? 3 - wave : wave;
   float fade[T::kStrips][4][4];
   if constexpr (MODE != kSums) {
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < T::kStrips; ++x) {
-      const int strip = x == 0 ? wave : 3 - wave;
+      const int strip = x == 0 ? strip0 : 3 - strip0;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          fade[x][kt][r] = s_power[max(16 * strip + (lane & 15) - (16 * kt + 4 * (lane >> 4) + r), 0)];
+          fade[x][kt][r] = s_power[max(16 * strip + (lane & 15) - (16 * kt + 4 * (lane >> 4) + r), 0)] *
+                           (kF16 ? 1.f : p.scale);
     }
   }
 
@@ -376,12 +428,15 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   auto load_tile = [&](const uint16_t* base, int64_t stride, uint32_t at, int64_t row0, int first) {
     const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
     Granules x;
-    if (first > 0) at = tid % T::kGranules * 16;
+    if (first == 0) {
 #pragma unroll
-    for (int i = 0; i < T::kLoads; ++i) {
-      uint32_t skip = 0;
-      if (first > 0) skip = static_cast<uint32_t>(max(16 * i + tile_row, first)) * static_cast<uint32_t>(stride * 2);
-      x.r[i] = *reinterpret_cast<const uint4*>(rows + (first > 0 ? 0 : i * 32 * stride) + (at + skip));
+      for (int i = 0; i < T::kLoads; ++i) x.r[i] = *reinterpret_cast<const uint4*>(rows + i * 32 * stride + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i)
+        x.r[i] = *reinterpret_cast<const uint4*>(
+            rows + (static_cast<uint32_t>(max(16 * i + tile_row, first)) * static_cast<uint32_t>(stride * 2) +
+                    tid % T::kGranules * 16));
     }
     return x;
   };
@@ -415,6 +470,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   Granules rq{};
   if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, q_lane, row0_of(0), first_of(0));
 
+  DecaySteps steps;
   for (int c = 0; c < chunks; ++c) {
     const int first = first_of(c);
     const int64_t row0 = row0_of(c);
@@ -424,18 +480,35 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     }
     store_tile(s_k, rk);
     store_tile(s_v, rv);
-    if constexpr (MODE != kSums) {
-      store_tile(s_q, rq);
-      bool wild = false;
+    if constexpr (MODE != kSums) store_tile(s_q, rq);
+    if constexpr (kF16) {
+      u16x2_t most = {0, 0};
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) wild |= any_wild<Tag>(rv.r[i]);
-      if (wild) s_wild = c + 1;
+      for (int i = 0; i < T::kLoads; ++i) most = max_bits(rv.r[i], most);
+      // As fp32 whole numbers they keep their order.
+      const int top = static_cast<int>(wave_max(static_cast<float>(max(most.x, most.y))));
+      if (lane == 0) atomicMax(&s_most[c & 1], top);
+    } else if constexpr (MODE != kSums) {
+      float zero = 0.f;
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) zero = add_zeros(rv.r[i], zero);
+      if (zero != zero) s_most[c & 1] = 1;
     }
     __syncthreads();
-    if (c + 1 < chunks) {
-      rk = load_tile(kn, p.k_stride, k_lane, row0_of(c + 1), first_of(c + 1));
-      rv = load_tile(vn, p.v_stride, v_lane, row0_of(c + 1), first_of(c + 1));
-    }
+    const int most = uniform(s_most[c & 1]);
+    if (tid == 0) s_most[(c + 1) & 1] = 0;  // last read before the barrier that ended chunk c - 1
+    // The next chunk's rows are asked for a tile at a time, between the phases of this one: all
+    // at once they fill the memory pipe and every wave waits to get its loads into it.
+    const bool more = c + 1 < chunks;
+    const int next_first = first_of(c + 1);
+    const int64_t next_row0 = row0_of(c + 1);
+    // The state's decay over the chunk; for f16 with v's scale taken out, which the update
+    // puts back.
+    const bool update = MODE == kSums || more || last;
+    Pow2 v_scale{1.f, 1.f};
+    if constexpr (kF16) v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(most)));
+    float fall = 1.f;
+    if (update) fall = steps.next(more ? over_chunk : over_last) * v_scale.down;
     if constexpr (MODE != kSums) {
       Pow2 s_scale{1.f, 1.f};
       if constexpr (kF16) {
@@ -453,39 +526,36 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           __syncthreads();
         }
         const bool same = g + 1 < p.group;  // the next tile of queries is this chunk's
-        if (same || c + 1 < chunks)
-          rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, q_lane, same ? row0 : row0_of(c + 1),
-                         same ? first : first_of(c + 1));
+        const float fall_now = same ? 1.f : fall;
 
         // Scores: K Q^T tiles, a query in each lane and four keys in its registers.
         const int r16 = fresh_copy(rows16), p16 = fresh_copy(scores16);
+        auto score_strip = [&](auto strip_constant, const float (&fade_x)[4][4]) {
+          constexpr int strip = decltype(strip_constant)::value;
+          uint4 qb[D / 32], kb[strip + 1][D / 32];
+          floatx4 score[4] = {};
 #pragma unroll
-        for (int x = 0; x < T::kStrips; ++x) {
-          const int strip = x == 0 ? wave : 3 - wave;
-          uint4 qb[D / 32];
+          for (int kk = 0; kk < D / 32; ++kk) {
+            qb[kk] = lds_read16(s_q + (r16 ^ (kk << 6)) + strip * T::kStep);
 #pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk) qb[kk] = lds_read16(s_q + (r16 ^ (kk << 6)) + strip * T::kStep);
-          floatx4 score[4];
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            score[kt] = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (kt <= strip) {
-#pragma unroll
-              for (int kk = 0; kk < D / 32; ++kk)
-                score[kt] = mfma16x16x32(Tag{}, lds_read16(s_k + (r16 ^ (kk << 6)) + kt * T::kStep), qb[kk], score[kt]);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const bool seen = kt < strip || 4 * (lane >> 4) + r <= (lane & 15);
-                score[kt][r] = seen ? score[kt][r] * fade[x][kt][r] : 0.f;
-              }
-            }
+            for (int kt = 0; kt <= strip; ++kt) kb[kt][kk] = lds_read16(s_k + (r16 ^ (kk << 6)) + kt * T::kStep);
           }
-          fence_schedule();
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+            for (int kt = 0; kt <= strip; ++kt) score[kt] = mfma16x16x32(Tag{}, kb[kt][kk], qb[kk], score[kt]);
+#pragma unroll
+          for (int kt = 0; kt <= strip; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool seen = kt < strip || 4 * (lane >> 4) + r <= (lane & 15);
+              score[kt][r] = seen ? score[kt][r] * fade_x[kt][r] : 0.f;
+            }
           Pow2 p_scale{1.f, 1.f};
           if constexpr (kF16) {
             float m = 0.f;
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
+            for (int kt = 0; kt <= strip; ++kt)
 #pragma unroll
               for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(score[kt][r]));
             p_scale = scale_for_f16(max_over_lane_groups(m));
@@ -493,40 +563,97 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           }
           // Tiles of keys behind the strip are read only where they share a block of 32.
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            if (kt > (strip | 1)) continue;
+          for (int kt = 0; kt <= (strip | 1); ++kt) {
             float y[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = kF16 ? score[kt][r] * p_scale.down : score[kt][r];
             *reinterpret_cast<uint2*>(s_p + (p16 ^ (kt << 5)) + strip * 16 * 128) =
                 make_uint2(pack2_cvt(Tag{}, y[0], y[1]), pack2_cvt(Tag{}, y[2], y[3]));
           }
+          fence_schedule();
+        };
+        if constexpr (T::kStrips == 1) {
+          switch (strip0) {
+            case 0: score_strip(Int<0>{}, fade[0]); break;
+            case 1: score_strip(Int<1>{}, fade[0]); break;
+            case 2: score_strip(Int<2>{}, fade[0]); break;
+            default: score_strip(Int<3>{}, fade[0]);
+          }
+        } else if (strip0 == 0) {
+          score_strip(Int<0>{}, fade[0]);
+          score_strip(Int<3>{}, fade[T::kStrips - 1]);
+        } else {
+          score_strip(Int<1>{}, fade[0]);
+          score_strip(Int<2>{}, fade[T::kStrips - 1]);
         }
-        __syncthreads();
 
-        fence_schedule();
+        if (same || more)
+          rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, q_lane, same ? row0 : next_row0,
+                         same ? first : next_first);
+
         // Outputs, transposed: a query (of both halves of the chunk) in each lane, value
-        // columns in its registers.
+        // columns in its registers.  First what the state gives, while other waves' scores
+        // are still to come; the next key rows' operands are read ahead.
+        fence_schedule();
         const int r32 = fresh_copy(rows32), p32 = fresh_copy(scores32);
         floatx16 acc[2];
 #pragma unroll
         for (int it = 0; it < 2; ++it)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[it][r] = 0.f;
+        uint4 qa[2][2];
+        auto read_queries = [&](int mt) {
 #pragma unroll
-        for (int mt = 0; mt < kMt; ++mt)
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int it = 0; it < 2; ++it)
+              qa[a][it] = lds_read16(s_q + (r32 ^ ((4 * mt + 2 * a) << 4)) + it * 2 * T::kStep);
+        };
+        uint4 s16[2];
+        auto pack_state = [&](int mt) {
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = kF16 ? S[mt][8 * a + i] * s_scale.down : S[mt][8 * a + i];
-            const uint4 s16 = pack8<Tag>(x);
-#pragma unroll
-            for (int it = 0; it < 2; ++it)
-              acc[it] = mfma32x32x16(Tag{}, s16, lds_read16(s_q + (r32 ^ ((4 * mt + 2 * a) << 4)) + it * 2 * T::kStep),
-                                     acc[it]);
-            fence_schedule();
+            s16[a] = pack8<Tag>(x);
           }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[mt][r] *= fall_now;
+        };
+        read_queries(0);
+        pack_state(0);
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          uint4 now[2][2], part[2];
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            part[a] = s16[a];
+#pragma unroll
+            for (int it = 0; it < 2; ++it) now[a][it] = qa[a][it];
+          }
+          if (mt + 1 < kMt) {
+            read_queries(mt + 1);
+            pack_state(mt + 1);
+          }
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int it = 0; it < 2; ++it) acc[it] = mfma32x32x16(Tag{}, part[a], now[a][it], acc[it]);
+          interleave<4, 4, 7>();
+          fence_schedule();
+        }
+        if (!same && more) rk = load_tile(kn, p.k_stride, k_lane, next_row0, next_first);
+        __syncthreads();
+
+        const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
+        uint4 v[4], ps[2][4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          v[kb] = columns_operand<D>(s_v, v0, v1, kb, wave);
+#pragma unroll
+          for (int it = kb / 2; it < 2; ++it) ps[it][kb] = lds_read16(s_p + (p32 ^ (kb << 5)) + it * 32 * 128);
+        }
         Pow2 p_scale[2] = {{1.f, 1.f}, {1.f, 1.f}};
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
@@ -536,21 +663,14 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
             p_scale[it].up = s_up[query];
             p_scale[it].down = __uint_as_float(0x7f000000u - __float_as_uint(p_scale[it].up));  // 1 / 2^e
             carry *= s_scale.up * p_scale[it].down;
+            p_scale[it].up *= p.scale;
+          } else {
+            carry *= p.scale;
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[it][r] *= carry;
         }
-        if (s_wild != c + 1) {
-          const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb) {
-            const uint4 v = columns_operand<D>(s_v, v0, v1, kb, wave);
-#pragma unroll
-            for (int it = kb / 2; it < 2; ++it)
-              acc[it] = mfma32x32x16(Tag{}, v, lds_read16(s_p + (p32 ^ (kb << 5)) + it * 32 * 128), acc[it]);
-            fence_schedule();
-          }
-        } else {
+        if (most >= (kF16 ? 0x7c00 : 1)) {  // one by one, and nothing left for the products
 #pragma unroll
           for (int it = 0; it < 2; ++it) {
             const int query = 32 * it + (lane & 31);
@@ -567,7 +687,13 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
               }
             }
           }
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) v[kb] = make_uint4(0, 0, 0, 0);
         }
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+          for (int it = kb / 2; it < 2; ++it) acc[it] = mfma32x32x16(Tag{}, v[kb], ps[it][kb], acc[it]);
         char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
@@ -577,8 +703,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
             for (int a = 0; a < 2; ++a) {
               float x[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                x[i] = (kF16 ? acc[it][8 * a + i] * p_scale[it].up : acc[it][8 * a + i]) * p.scale;
+              for (int i = 0; i < 8; ++i) x[i] = kF16 ? acc[it][8 * a + i] * p_scale[it].up : acc[it][8 * a + i];
               *reinterpret_cast<uint4*>(out + it * 32 * static_cast<int64_t>(p.num_heads * D * 2) + out_lane + 32 * a) =
                   pack8<Tag>(x);
             }
@@ -589,38 +714,29 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     }
 
     fence_schedule();
-    if (MODE == kSums || c + 1 < chunks || last) {
-      Decay fall = c + 1 < chunks ? over_chunk : over_last;
-      Pow2 v_scale{1.f, 1.f};
+    if (more) {
+      if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, k_lane, next_row0, next_first);
+      rv = load_tile(vn, p.v_stride, v_lane, next_row0, next_first);
+    }
+    if (update) {
       const int k0 = fresh_copy(cols0), k1 = fresh_copy(cols1);
-      if constexpr (kF16) {
-        float m = 0.f;
+      if constexpr (MODE == kSums) {
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          float x[8];
-          unpack8<Tag>(columns_operand<D>(s_v, k0, k1, kb, wave), x);
+        for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-        }
-        v_scale = scale_for_f16(wave_max(m));
-        fall.hi *= v_scale.down;
-        fall.lo *= v_scale.down;
+          for (int r = 0; r < 16; ++r) S[mt][r] *= fall;
       }
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) S[mt][r] = fall * S[mt][r];
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
+      // The products of 16 tokens, while the next 16's operands are read and weighted.
+      constexpr int kTerms = kF16 ? 2 : 3;
+      uint4 term[kTerms], k[kMt];
+      auto weigh = [&](uint4 v, int kb) {
         float x[8], y[8];
-        unpack8<Tag>(columns_operand<D>(s_v, k0, k1, kb, wave), x);
+        unpack8<Tag>(v, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] *= s_weight[16 * kb + 8 * half + i];
           if constexpr (kF16) x[i] *= v_scale.down;
         }
-        constexpr int kTerms = kF16 ? 2 : 3;
-        uint4 term[kTerms];
 #pragma unroll
         for (int t = 0; t < kTerms; ++t) {
           term[t] = pack8<Tag>(x);
@@ -628,12 +744,31 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] -= y[i];
         }
+      };
+      uint4 v = columns_operand<D>(s_v, k0, k1, 0, wave);
 #pragma unroll
-        for (int mt = 0; mt < kMt; ++mt) {
-          const uint4 k = columns_operand<D>(s_k, k0, k1, kb, mt);
+      for (int mt = 0; mt < kMt; ++mt) k[mt] = columns_operand<D>(s_k, k0, k1, 0, mt);
+      weigh(v, 0);
+      v = columns_operand<D>(s_v, k0, k1, 1, wave);
 #pragma unroll
-          for (int t = 0; t < kTerms; ++t) S[mt] = mfma32x32x16(Tag{}, k, term[t], S[mt]);
+      for (int kb = 0; kb < 4; ++kb) {
+        uint4 now[kMt], part[kTerms];
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) now[mt] = k[mt];
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) part[t] = term[t];
+        const uint4 v_next = v;
+        if (kb < 2) v = columns_operand<D>(s_v, k0, k1, kb + 2, wave);
+        if (kb < 3) {
+#pragma unroll
+          for (int mt = 0; mt < kMt; ++mt) k[mt] = columns_operand<D>(s_k, k0, k1, kb + 1, mt);
         }
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t)
+#pragma unroll
+          for (int mt = 0; mt < kMt; ++mt) S[mt] = mfma32x32x16(Tag{}, now[mt], part[t], S[mt]);
+        if (kb < 3) weigh(v_next, kb + 1);
+        interleave<2 * kMt + 2, kTerms * kMt, 6>();
         fence_schedule();
       }
       if constexpr (kF16) {
