@@ -423,18 +423,18 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   // Rows from `first` (of the chunk) on hold tokens; in place of those before, row `first`
   // is read, and zeros are stored for k and v.
   struct Granules {
-    uint4 r[T::kLoads];
+    oxide::u32x4 r[T::kLoads];
   };
   auto load_tile = [&](const uint16_t* base, int64_t stride, uint32_t at, int64_t row0, int first) {
     const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
     Granules x;
     if (first == 0) {
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) x.r[i] = *reinterpret_cast<const uint4*>(rows + i * 32 * stride + at);
+      for (int i = 0; i < T::kLoads; ++i) x.r[i] = *reinterpret_cast<const oxide::u32x4*>(rows + i * 32 * stride + at);
     } else {
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i)
-        x.r[i] = *reinterpret_cast<const uint4*>(
+        x.r[i] = *reinterpret_cast<const oxide::u32x4*>(
             rows + (static_cast<uint32_t>(max(16 * i + tile_row, first)) * static_cast<uint32_t>(stride * 2) +
                     tid % T::kGranules * 16));
     }
@@ -442,12 +442,21 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   };
   auto store_tile = [&](char* tile, const Granules& x) {
 #pragma unroll
-    for (int i = 0; i < T::kLoads; ++i) *reinterpret_cast<uint4*>(tile + tile_at + i * T::kStep) = x.r[i];
+    for (int i = 0; i < T::kLoads; ++i) *reinterpret_cast<oxide::u32x4*>(tile + tile_at + i * T::kStep) = x.r[i];
+  };
+  // Loaded rows are first looked at here: otherwise what the next chunk does with them is
+  // begun where they are asked for, with a wait for memory.
+  auto arrived = [&](Granules x) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      asm volatile("" : "+v"(x.r[i]));
+    }
+    return x;
   };
   auto without_padding = [&](Granules x, int first) {
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i)
-      if (16 * i + tile_row < first) x.r[i] = make_uint4(0, 0, 0, 0);
+      if (16 * i + tile_row < first) x.r[i] = oxide::u32x4{0, 0, 0, 0};
     return x;
   };
 
@@ -474,24 +483,26 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   for (int c = 0; c < chunks; ++c) {
     const int first = first_of(c);
     const int64_t row0 = row0_of(c);
+    rk = arrived(rk);
+    rv = arrived(rv);
     if (first > 0) {
       rk = without_padding(rk, first);
       rv = without_padding(rv, first);
     }
     store_tile(s_k, rk);
     store_tile(s_v, rv);
-    if constexpr (MODE != kSums) store_tile(s_q, rq);
+    if constexpr (MODE != kSums) store_tile(s_q, arrived(rq));
     if constexpr (kF16) {
       u16x2_t most = {0, 0};
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) most = max_bits(rv.r[i], most);
+      for (int i = 0; i < T::kLoads; ++i) most = max_bits(__builtin_bit_cast(uint4, rv.r[i]), most);
       // As fp32 whole numbers they keep their order.
       const int top = static_cast<int>(wave_max(static_cast<float>(max(most.x, most.y))));
       if (lane == 0) atomicMax(&s_most[c & 1], top);
     } else if constexpr (MODE != kSums) {
       float zero = 0.f;
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) zero = add_zeros(rv.r[i], zero);
+      for (int i = 0; i < T::kLoads; ++i) zero = add_zeros(__builtin_bit_cast(uint4, rv.r[i]), zero);
       if (zero != zero) s_most[c & 1] = 1;
     }
     __syncthreads();
@@ -522,7 +533,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 
       for (int g = 0; g < p.group; ++g) {
         if (g > 0) {
-          store_tile(s_q, rq);
+          store_tile(s_q, arrived(rq));
           __syncthreads();
         }
         const bool same = g + 1 < p.group;  // the next tile of queries is this chunk's
