@@ -307,14 +307,22 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ float uniform(float x) { return __int_as_float(uniform(__float_as_int(x))); }
 __device__ __forceinline__ Decay uniform(Decay d) { return Decay{uniform(d.hi), uniform(d.lo)}; }
 
-// A sequence's rows: at most max_q, and none past the last there is.
-struct Rows {
-  int begin, end;
+// A sequence's slot, rows (at most max_q, and none past the last there is) and whether it
+// starts from zero, and a head's decay: asked for together, before any is looked at.
+struct Sequence {
+  int slot, begin, end;
+  bool fresh;
+  float log_decay;
 };
-__device__ __forceinline__ Rows rows_of(const LinearParams& p, int b) {
-  const int64_t begin = min(static_cast<int64_t>(p.cu_q[b]), p.total_q);
-  const int64_t end = min(min(static_cast<int64_t>(p.cu_q[b + 1]), p.total_q), begin + p.max_q);
-  return Rows{static_cast<int>(begin), static_cast<int>(end)};
+__device__ __forceinline__ Sequence sequence_of(const LinearParams& p, int b, int n) {
+  const int slot = p.slots[b];
+  const uint32_t from = p.cu_q[b], to = p.cu_q[b + 1];
+  const uint32_t context = *(p.context_lens ? p.context_lens + b : p.cu_q);
+  const float log_decay = p.log_decay[n];
+  const int64_t begin = min(static_cast<int64_t>(from), p.total_q);
+  const int64_t end = min(min(static_cast<int64_t>(to), p.total_q), begin + p.max_q);
+  return Sequence{uniform(slot), uniform(static_cast<int>(begin)), uniform(static_cast<int>(end)),
+                  p.context_lens && uniform(static_cast<int>(context)) == 0, uniform(log_decay)};
 }
 
 // What a launch does with its pieces of sequences.
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   __shared__ char s_v[T::kTileBytes] __attribute__((aligned(16)));
   __shared__ char s_q[MODE == kSums ? 16 : T::kTileBytes] __attribute__((aligned(16)));
   __shared__ char s_p[MODE == kSums ? 16 : kChunk * 128] __attribute__((aligned(16)));
-  __shared__ float s_power[kChunk + 1];                            // lambda^m
+  __shared__ float s_power[kChunk + 1], s_power_low[kChunk + 1];   // lambda^m, and what its rounding leaves
   __shared__ float s_weight[kChunk] __attribute__((aligned(16)));  // lambda^(63 - j)
   __shared__ float s_up[kChunk];                                   // f16: 2^e of P's rows
   // Of even and odd chunks: bf16, whether v holds an infinity or NaN; f16, its largest
@@ -344,10 +352,10 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const int n = blockIdx.x % p.num_kv_heads;
   const int piece = MODE == kWhole ? 0 : blockIdx.x / p.num_kv_heads % p.pieces;
   const int b = blockIdx.x / p.num_kv_heads / (MODE == kWhole ? 1 : p.pieces);
-  const int64_t slot = p.slots[b];
+  const Sequence seq = sequence_of(p, b, n);
+  const int slot = seq.slot, begin = seq.begin, end = seq.end;
+  const float ld = seq.log_decay;
   if (slot < 0 || slot >= p.num_slots) return;
-  const Rows rows = rows_of(p, b);
-  const int begin = uniform(rows.begin), end = uniform(rows.end);
   const int t0 = begin + (MODE == kWhole ? 0 : min(end - begin, piece * p.piece_tokens));
   if (t0 >= end) return;
   const int t1 = MODE == kWhole ? end : t0 + min(end - t0, p.piece_tokens);
@@ -358,61 +366,9 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const int64_t unit = MODE == kWhole ? 0 : begin / p.piece_tokens + piece - (MODE == kPieces ? 1 : 0);
   if (MODE == kSums && unit >= p.units) return;
   float* const ws = p.workspace + (unit * p.num_kv_heads + n) * D * D + tid * 4;
-  float* const state = p.state + (slot * p.num_kv_heads + n) * D * D + 32 * wave + deal(lane & 31);
-
-  const float ld = p.log_decay[n];
+  float* const state =
+      p.state + (static_cast<int64_t>(slot) * p.num_kv_heads + n) * D * D + 32 * wave + deal(lane & 31);
   const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
-  for (int m = tid; m <= kChunk; m += T::kThreads) {
-    const float x = decay_power(ld, m).hi;
-    s_power[m] = x;
-    if (m < kChunk) s_weight[kChunk - 1 - m] = x;
-  }
-  if (tid < 2) s_most[tid] = 0;
-  const Decay over_chunk = uniform(decay_power(ld, kChunk));
-  const Decay over_last = uniform(decay_power(ld, t1 - t0 - (chunks - 1) * kChunk));
-
-  // Lane's state values: register 8 a + i of tile mt is key row 32 mt + 16 a + 8 half + i.
-  floatx16 S[kMt];
-#pragma unroll
-  for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) S[mt][r] = 0.f;
-  if (MODE == kPieces && piece > 0) {
-    if (unit < p.units) {
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[mt][r + e] = x[e];
-        }
-    }
-  } else if (MODE != kSums && !(p.context_lens && p.context_lens[b] == 0)) {
-#pragma unroll
-    for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
-  }
-
-  // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
-  // Strips have one to four tiles of keys: of two workgroups on a compute unit (neighbours in
-  // the grid 8 or 256 apart) one deals them out in reverse, so that its SIMDs get even work.
-  const int strip0 = T::kStrips == 1 && ((blockIdx.x >> 3 ^ blockIdx.x >> 8) & 1) ? 3 - wave : wave;
-  float fade[T::kStrips][4][4];
-  if constexpr (MODE != kSums) {
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < T::kStrips; ++x) {
-      const int strip = x == 0 ? strip0 : 3 - strip0;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          fade[x][kt][r] = s_power[max(16 * strip + (lane & 15) - (16 * kt + 4 * (lane >> 4) + r), 0)] *
-                           (kF16 ? 1.f : p.scale);
-    }
-  }
 
   // A thread moves granule tid % kGranules of rows tid / kGranules + 16 i of a tile.
   const int tile_row = tid / T::kGranules, tile_at = T::at(tile_row, tid % T::kGranules);
@@ -467,6 +423,62 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   auto first_of = [&](int c) { return c + 1 < chunks ? 0 : chunks * kChunk - (t1 - t0); };
   auto row0_of = [&](int c) { return static_cast<int64_t>(t0) + c * kChunk - first_of(c); };
 
+  Granules rk = load_tile(kn, p.k_stride, k_lane, row0_of(0), first_of(0));
+  Granules rv = load_tile(vn, p.v_stride, v_lane, row0_of(0), first_of(0));
+  Granules rq{};
+  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, q_lane, row0_of(0), first_of(0));
+
+  for (int m = tid; m <= kChunk; m += T::kThreads) {
+    const Decay x = decay_power(ld, m);
+    s_power[m] = x.hi;
+    s_power_low[m] = x.lo;
+    if (m < kChunk) s_weight[kChunk - 1 - m] = x.hi;
+  }
+  if (tid < 2) s_most[tid] = 0;
+
+  // Lane's state values: register 8 a + i of tile mt is key row 32 mt + 16 a + 8 half + i.
+  floatx16 S[kMt];
+#pragma unroll
+  for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[mt][r] = 0.f;
+  if (MODE == kPieces && piece > 0) {
+    if (unit < p.units) {
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const floatx4 x = *reinterpret_cast<const floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[mt][r + e] = x[e];
+        }
+    }
+  } else if (MODE != kSums && !seq.fresh) {
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
+  }
+
+  // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
+  // Strips have one to four tiles of keys: of two workgroups on a compute unit (neighbours in
+  // the grid 8 or 256 apart) one deals them out in reverse, so that its SIMDs get even work.
+  const int strip0 = T::kStrips == 1 && ((blockIdx.x >> 3 ^ blockIdx.x >> 8) & 1) ? 3 - wave : wave;
+  float fade[T::kStrips][4][4];
+  __syncthreads();
+  if constexpr (MODE != kSums) {
+#pragma unroll
+    for (int x = 0; x < T::kStrips; ++x) {
+      const int strip = x == 0 ? strip0 : 3 - strip0;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          fade[x][kt][r] = s_power[max(16 * strip + (lane & 15) - (16 * kt + 4 * (lane >> 4) + r), 0)] *
+                           (kF16 ? 1.f : p.scale);
+    }
+  }
+
   // Offsets of the lane's operands in the tiles.
   const int rows16 = T::at(lane & 15, lane >> 4), rows32 = T::at(lane & 31, half);
   const int cols0 = columns_at<D>(lane, 0), cols1 = columns_at<D>(lane, 1);
@@ -474,11 +486,9 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const uint32_t out_lane = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(p.num_heads * D * 2) +
                             (32 * wave + 8 * half) * 2;
 
-  Granules rk = load_tile(kn, p.k_stride, k_lane, row0_of(0), first_of(0));
-  Granules rv = load_tile(vn, p.v_stride, v_lane, row0_of(0), first_of(0));
-  Granules rq{};
-  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, q_lane, row0_of(0), first_of(0));
-
+  const int in_last = t1 - t0 - (chunks - 1) * kChunk;
+  const Decay over_chunk = uniform(Decay{s_power[kChunk], s_power_low[kChunk]});
+  const Decay over_last = uniform(Decay{s_power[in_last], s_power_low[in_last]});
   DecaySteps steps;
   for (int c = 0; c < chunks; ++c) {
     const int first = first_of(c);
@@ -815,33 +825,46 @@ __global__ __launch_bounds__(256) void linear_prefill_join(LinearParams p) {
   using T = Tiles<D>;
   constexpr int kQuads = D * D / 4;
   const int blocks = kQuads / 256;
-  const int quad = blockIdx.x % blocks * 256 + threadIdx.x;
-  const int n = blockIdx.x / blocks % p.num_kv_heads;
-  const int b = blockIdx.x / blocks / p.num_kv_heads;
-  const int64_t slot = p.slots[b];
+  // Heads run fastest in all three grids: with kv heads a multiple of the eight XCDs, a
+  // head's pieces, and with them what the workspace holds of it, stay on one.
+  const int n = blockIdx.x % p.num_kv_heads;
+  const int quad = blockIdx.x / p.num_kv_heads % blocks * 256 + threadIdx.x;
+  const int b = blockIdx.x / p.num_kv_heads / blocks;
+  const Sequence seq = sequence_of(p, b, n);
+  const int slot = seq.slot, begin = seq.begin;
   if (slot < 0 || slot >= p.num_slots) return;
-  const Rows rows = rows_of(p, b);
-  const int begin = rows.begin;
-  const int sums = rows.end > begin ? (rows.end - begin - 1) / p.piece_tokens : 0;  // all pieces but the last
-  if (sums == 0) return;
+  const int sums = seq.end > begin ? (seq.end - begin - 1) / p.piece_tokens : 0;  // all pieces but the last
+  if (sums == 0 || begin / p.piece_tokens >= p.units) return;
   // Where the workspace's quad lies in the state (as linear_prefill_chunks keeps it).
   const int tid = quad % T::kThreads, part = quad / T::kThreads, lane = tid & 63;
   const int row = 32 * (part / 4) + 16 * (part % 4 / 2) + 8 * (lane >> 5) + 4 * (part % 2);
   const int col = 32 * (tid >> 6) + deal(lane & 31);
   floatx4 s = {0.f, 0.f, 0.f, 0.f};
-  if (!(p.context_lens && p.context_lens[b] == 0)) {
-    const float* state = p.state + (slot * p.num_kv_heads + n) * D * D + row * D + col;
+  if (!seq.fresh) {
+    const float* state = p.state + (static_cast<int64_t>(slot) * p.num_kv_heads + n) * D * D + row * D + col;
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = state[e * D];
   }
-  const Decay fall = decay_power(p.log_decay[n], p.piece_tokens);
+  const Decay fall = decay_power(seq.log_decay, p.piece_tokens);
   const int64_t first = begin / p.piece_tokens;
-  for (int i = 0; i < sums && first + i < p.units; ++i) {
-    float* ws = p.workspace + ((first + i) * p.num_kv_heads + n) * D * D + quad * 4;
-    const floatx4 add = *reinterpret_cast<const floatx4*>(ws);
+  const int count = static_cast<int>(min(static_cast<int64_t>(sums), p.units - first));
+  const int64_t step = static_cast<int64_t>(p.num_kv_heads) * D * D;
+  float* const ws = p.workspace + (first * p.num_kv_heads + n) * D * D + quad * 4;
+  constexpr int kAhead = 4;  // sums asked for before the first is needed
+  floatx4 next[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fall * s[e] + add[e];
-    *reinterpret_cast<floatx4*>(ws) = s;
+  for (int a = 0; a < kAhead; ++a) next[a] = *reinterpret_cast<const floatx4*>(ws + min(a, count - 1) * step);
+  for (int i0 = 0; i0 < count; i0 += kAhead) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const floatx4 add = next[a];
+      next[a] = *reinterpret_cast<const floatx4*>(ws + min(i0 + a + kAhead, count - 1) * step);
+      if (i0 + a < count) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = fall * s[e] + add[e];
+        *reinterpret_cast<floatx4*>(ws + (i0 + a) * step) = s;
+      }
+    }
   }
 }
 
