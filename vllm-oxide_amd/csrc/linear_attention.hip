@@ -490,6 +490,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const Decay over_chunk = uniform(Decay{s_power[kChunk], s_power_low[kChunk]});
   const Decay over_last = uniform(Decay{s_power[in_last], s_power_low[in_last]});
   DecaySteps steps;
+  float s_unit = 1.f;
   for (int c = 0; c < chunks; ++c) {
     const int first = first_of(c);
     const int64_t row0 = row0_of(c);
@@ -523,13 +524,13 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     const bool more = c + 1 < chunks;
     const int next_first = first_of(c + 1);
     const int64_t next_row0 = row0_of(c + 1);
-    // The state's decay over the chunk; for f16 with v's scale taken out, which the update
-    // puts back.
+    // The state's decay over the chunk.  f16: what is added to it comes scaled by v's power
+    // of two, so the registers hold the state over `s_unit`.
     const bool update = MODE == kSums || more || last;
     Pow2 v_scale{1.f, 1.f};
     if constexpr (kF16) v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(most)));
     float fall = 1.f;
-    if (update) fall = steps.next(more ? over_chunk : over_last) * v_scale.down;
+    if (update) fall = steps.next(more ? over_chunk : over_last) * (kF16 ? s_unit * v_scale.down : 1.f);
     if constexpr (MODE != kSums) {
       Pow2 s_scale{1.f, 1.f};
       if constexpr (kF16) {
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(S[mt][r]));
-        s_scale = scale_for_f16(wave_max(m));
+        s_scale = scale_for_f16(wave_max(m));  // of the registers' values
       }
 
       for (int g = 0; g < p.group; ++g) {
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           if constexpr (kF16) {
             p_scale[it].up = s_up[query];
             p_scale[it].down = __uint_as_float(0x7f000000u - __float_as_uint(p_scale[it].up));  // 1 / 2^e
-            carry *= s_scale.up * p_scale[it].down;
+            carry *= s_scale.up * s_unit * p_scale[it].down;
             p_scale[it].up *= p.scale;
           } else {
             carry *= p.scale;
@@ -792,16 +793,17 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         interleave<2 * kMt + 2, kTerms * kMt, 6>();
         fence_schedule();
       }
-      if constexpr (kF16) {
-#pragma unroll
-        for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) S[mt][r] *= v_scale.up;
-      }
+      if constexpr (kF16) s_unit = v_scale.up;
     }
     __syncthreads();
   }
 
+  if constexpr (kF16) {
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[mt][r] *= s_unit;
+  }
   if (MODE == kSums) {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
