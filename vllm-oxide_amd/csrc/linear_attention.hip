@@ -483,8 +483,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const int rows16 = T::at(lane & 15, lane >> 4), rows32 = T::at(lane & 31, half);
   const int cols0 = columns_at<D>(lane, 0), cols1 = columns_at<D>(lane, 1);
   const int scores16 = T::score_at(lane & 15, half) + ((lane >> 4) & 1) * 8, scores32 = T::score_at(lane & 31, half);
-  const uint32_t out_lane = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(p.num_heads * D * 2) +
-                            (32 * wave + 8 * half) * 2;
+  const uint32_t out_lane = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
 
   const int in_last = t1 - t0 - (chunks - 1) * kChunk;
   const Decay over_chunk = uniform(Decay{s_power[kChunk], s_power_low[kChunk]});
@@ -522,6 +521,16 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     // The next chunk's rows are asked for a tile at a time, between the phases of this one: all
     // at once they fill the memory pipe and every wave waits to get its loads into it.
     const bool more = c + 1 < chunks;
+    // A thread moves the granules of the output tile in whose place it puts the next queries.
+    auto store_out = [&](int g) {
+      char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) {
+        const oxide::u32x4 x = *reinterpret_cast<const oxide::u32x4*>(s_q + tile_at + i * T::kStep);
+        if (16 * i + tile_row >= first)
+          *reinterpret_cast<oxide::u32x4*>(out + i * 16 * static_cast<int64_t>(p.num_heads * D * 2) + out_lane) = x;
+      }
+    };
     const int next_first = first_of(c + 1);
     const int64_t next_row0 = row0_of(c + 1);
     // The state's decay over the chunk.  f16: what is added to it comes scaled by v's power
@@ -543,10 +552,6 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       }
 
       for (int g = 0; g < p.group; ++g) {
-        if (g > 0) {
-          store_tile(s_q, arrived(rq));
-          __syncthreads();
-        }
         const bool same = g + 1 < p.group;  // the next tile of queries is this chunk's
         const float fall_now = same ? 1.f : fall;
 
@@ -716,22 +721,23 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
           for (int it = kb / 2; it < 2; ++it) acc[it] = mfma32x32x16(Tag{}, v[kb], ps[it][kb], acc[it]);
-        char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+        // Into the place of the queries, which every wave is done with: rows then leave whole,
+        // 256 bytes at a time, instead of 16 bytes of 64 rows by each wave.
 #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          const int query = 32 * it + (lane & 31);
-          if (query >= first) {
+        for (int it = 0; it < 2; ++it)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              float x[8];
+          for (int a = 0; a < 2; ++a) {
+            float x[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = kF16 ? acc[it][8 * a + i] * p_scale[it].up : acc[it][8 * a + i];
-              *reinterpret_cast<uint4*>(out + it * 32 * static_cast<int64_t>(p.num_heads * D * 2) + out_lane + 32 * a) =
-                  pack8<Tag>(x);
-            }
+            for (int i = 0; i < 8; ++i) x[i] = kF16 ? acc[it][8 * a + i] * p_scale[it].up : acc[it][8 * a + i];
+            *reinterpret_cast<uint4*>(s_q + (r32 ^ ((4 * wave + 2 * a) << 4)) + it * 2 * T::kStep) = pack8<Tag>(x);
           }
+        if (same) {
+          __syncthreads();
+          store_out(g);
+          store_tile(s_q, arrived(rq));
+          __syncthreads();
         }
-        if (g + 1 < p.group) __syncthreads();
       }
     }
 
@@ -796,6 +802,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       if constexpr (kF16) s_unit = v_scale.up;
     }
     __syncthreads();
+    if constexpr (MODE != kSums) store_out(p.group - 1);
   }
 
   if constexpr (kF16) {
