@@ -40,6 +40,7 @@ struct LinearParams {
   int64_t units;  // states of each kv head in the workspace
   int batch, num_heads, num_kv_heads, group, max_q;
   int piece_tokens, pieces;  // tokens of a piece, pieces of the longest sequence
+  bool joined;  // the workspace holds the states at the pieces' begins, not the pieces' sums
   float scale;
 };
 
@@ -442,27 +443,32 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[mt][r] = 0.f;
-  if (MODE == kPieces && piece > 0) {
-    if (unit < p.units) {
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[mt][r + e] = x[e];
-        }
-    }
-  } else if (MODE != kSums && !seq.fresh) {
+  if (MODE != kSums && !seq.fresh && (MODE == kWhole || piece == 0 || !p.joined)) {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
   }
+  if (MODE == kPieces && piece > 0 && unit < p.units) {
+    // The state at the piece's begin, or the earlier pieces' sums one after the other.
+    const Decay over_piece = decay_power(ld, p.piece_tokens);
+    for (int back = p.joined ? 0 : piece - 1; back >= 0; --back) {
+      const float* from = ws - static_cast<int64_t>(back) * p.num_kv_heads * D * D;
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const floatx4 x = *reinterpret_cast<const floatx4*>(from + (mt * 4 + r / 4) * T::kThreads * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[mt][r + e] = p.joined ? x[e] : over_piece * S[mt][r + e] + x[e];
+        }
+    }
+  }
 
-  // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16, keys 16 kt + 4 (lane / 16) + r.
-  // Strips have one to four tiles of keys: of two workgroups on a compute unit (neighbours in
-  // the grid 8 or 256 apart) one deals them out in reverse, so that its SIMDs get even work.
+  // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16,
+  // keys 16 kt + 4 (lane / 16) + r.  Strips have one to four tiles of keys: of two workgroups
+  // on a compute unit (neighbours in the grid 8 or 256 apart) one deals them out in reverse,
+  // so that its SIMDs get even work.
   const int strip0 = T::kStrips == 1 && ((blockIdx.x >> 3 ^ blockIdx.x >> 8) & 1) ? 3 - wave : wave;
   float fade[T::kStrips][4][4];
   __syncthreads();
@@ -1036,7 +1042,11 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
     p.pieces = static_cast<int>((p.max_q + plan.piece_tokens - 1) / plan.piece_tokens);
     const dim3 grid(heads * static_cast<unsigned>(p.pieces));
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kSums>), grid, threads, 0, s, p);
-    hipLaunchKernelGGL((linear_prefill_join<D>), dim3(heads * (D * D / 4 / 256)), dim3(256), 0, s, p);
+    // A piece adds up the sums before it by itself where they are few: over P pieces that
+    // reads P (P - 1) / 2 states, where joining first moves 3 (P - 1) and is a launch more.
+    p.joined = p.pieces > 6;
+    if (p.joined)
+      hipLaunchKernelGGL((linear_prefill_join<D>), dim3(heads * (D * D / 4 / 256)), dim3(256), 0, s, p);
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), grid, threads, 0, s, p);
   });
   oxide::check_launch();
