@@ -11,6 +11,7 @@
 // column, then over the waves through LDS.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "cdna4_tile.hpp"
@@ -893,11 +894,14 @@ Plan plan_prefill(int64_t total_q, int64_t batch, int64_t num_heads, int64_t num
   if (total_q <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128) || max_seqlen_q <= 0)
     return whole;
-  const int64_t wanted = 2 * oxide::device_cu_count();  // workgroups
-  if (batch * num_kv_heads >= wanted) return whole;
-  int64_t piece = (total_q * num_kv_heads + wanted - 1) / wanted;
+  // As many pieces as workgroups are resident (LDS and registers hold two on a compute unit
+  // at D = 128, four at 64), but none whose rows are fewer bytes than its state costs
+  // (written, joined, read: 16 D^2, against 4 D (1 + group) a token).
+  const int64_t resident = (head_dim == 128 ? 2 : 4) * oxide::device_cu_count();
+  const int64_t group = num_heads / num_kv_heads;
+  int64_t piece = (total_q * num_kv_heads + resident - 1) / resident;
+  piece = std::max(piece, 4 * head_dim / (1 + group));
   piece = (piece + kChunk - 1) / kChunk * kChunk;
-  if (piece < 256) piece = 256;
   if (max_seqlen_q <= 2 * piece) return whole;
   return Plan{piece, total_q / piece};
 }
@@ -1044,7 +1048,7 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kSums>), grid, threads, 0, s, p);
     // A piece adds up the sums before it by itself where they are few: over P pieces that
     // reads P (P - 1) / 2 states, where joining first moves 3 (P - 1) and is a launch more.
-    p.joined = p.pieces > 6;
+    p.joined = p.pieces > 8;
     if (p.joined)
       hipLaunchKernelGGL((linear_prefill_join<D>), dim3(heads * (D * D / 4 / 256)), dim3(256), 0, s, p);
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), grid, threads, 0, s, p);
