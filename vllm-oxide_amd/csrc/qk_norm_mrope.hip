@@ -58,7 +58,6 @@ struct MropeParams {
   int num_heads;
   int num_kv_heads;
   int rounds;  // of kHeads heads that a wave walks
-  int parts;   // waves that share a token
   float eps;
   uint32_t axis[4];  // axis of frequency j: bits 2 (j % 16) of word j / 16
 };
@@ -139,28 +138,36 @@ __global__ __launch_bounds__(kMropeThreads) void qk_norm_mrope_cache_kernel(Mrop
   constexpr int kHeads = 64 / kLanes;   // that a wave holds at once
   const int lane = threadIdx.x & 63;
   const int sub = lane % kLanes;
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kMropeThreads / 64) + (threadIdx.x >> 6);
-  const int64_t t = wave / p.parts;
+  // The wave's token, positions and slot are scalars.
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kMropeThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= p.num_tokens) return;
   const int q_heads = p.num_heads, qk_heads = p.num_heads + p.num_kv_heads, heads = qk_heads + p.num_kv_heads;
   const uint16_t* row = p.qkv + t * p.qkv_stride;
-  int h = static_cast<int>(wave - t * p.parts) * p.rounds * kHeads + lane / kLanes;
+  int h = static_cast<int>(blockIdx.y) * p.rounds * kHeads + lane / kLanes;
   const int end = min(heads, h - lane / kLanes + p.rounds * kHeads);
 
-  // Past the last head a lane reads the last head's row and writes nothing.
-  Slices next = load_slices<D, V, true>(row + static_cast<int64_t>(min(h, heads - 1)) * D, sub);
-  int64_t slot = p.slot_mapping ? p.slot_mapping[t] : -1;
-  if (slot >= p.num_slots) slot = -1;
-  const uint32_t owner = p.axis[sub / 2] >> (16 * (sub & 1));
+  // Positions first: the table's rows wait for them, and loads return in order.
   int32_t pos[kMaxAxes];
 #pragma unroll
-  for (int a = 0; a < kMaxAxes; ++a)
-    pos[a] = a < p.num_axes ? min(max(p.positions[a * p.num_tokens + t], 0), p.max_position - 1) : 0;
+  for (int a = 0; a < kMaxAxes; ++a) pos[a] = p.positions[min(a, p.num_axes - 1) * p.num_tokens + t];
+  int64_t slot = *(p.slot_mapping ? p.slot_mapping + t : reinterpret_cast<const int64_t*>(p.cos_sin));
+  // Past the last head a lane reads the last head's row and writes nothing.
+  Slices next = load_slices<D, V, true>(row + static_cast<int64_t>(min(h, heads - 1)) * D, sub);
+  if (!p.slot_mapping || slot >= p.num_slots) slot = -1;
+  uint32_t owner = p.axis[0];
+#pragma unroll
+  for (int w = 1; w < D / 32; ++w) owner = sub / 2 == w ? p.axis[w] : owner;
+  owner >>= 16 * (sub & 1);
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) pos[a] = min(max(pos[a], 0), p.max_position - 1);
   float c[E], s[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const uint32_t a = (owner >> (2 * e)) & 3u;
-    const int at = a == 0 ? pos[0] : a == 1 ? pos[1] : a == 2 ? pos[2] : pos[3];
+    int at = pos[0];
+#pragma unroll
+    for (int b = 1; b < kMaxAxes; ++b) at = a == static_cast<uint32_t>(b) ? pos[b] : at;
     const float* cs = p.cos_sin + static_cast<int64_t>(at) * D + sub * E + e;
     c[e] = cs[0];
     s[e] = cs[D / 2];
@@ -213,10 +220,12 @@ template <class Tag, int D>
 void launch_mrope(MropeParams p, bool vec, hipStream_t s) {
   constexpr int kHeads = 64 / (D / 16);
   const int rounds = (p.num_heads + 2 * p.num_kv_heads + kHeads - 1) / kHeads;
-  p.parts = 1;
-  p.rounds = (rounds + p.parts - 1) / p.parts;
-  const int64_t waves = p.num_tokens * p.parts;
-  const dim3 grid(static_cast<unsigned>((waves + kMropeThreads / 64 - 1) / (kMropeThreads / 64)));
+  // A wave for a token's heads, or for a round of them where that leaves most of the chip
+  // idle: 5.9 against 7.2 us at 64 tokens of 32 + 8 + 8 heads, 149 against 70 at 16k.
+  const int parts = static_cast<int>(std::min<int64_t>(rounds, std::max<int64_t>(1, 2048 / p.num_tokens)));
+  p.rounds = (rounds + parts - 1) / parts;
+  const dim3 grid(static_cast<unsigned>((p.num_tokens + kMropeThreads / 64 - 1) / (kMropeThreads / 64)),
+                  static_cast<unsigned>((rounds + p.rounds - 1) / p.rounds));
   if (vec)
     hipLaunchKernelGGL((qk_norm_mrope_cache_kernel<Tag, D, true>), grid, dim3(kMropeThreads), 0, s, p);
   else
