@@ -25,13 +25,19 @@ _HEADS = ((16, 8), (32, 8), (40, 8), (64, 8), (28, 4))
 _LINEAR_HEADS = ((16, 16), (32, 32), (8, 8), (32, 8), (28, 4), (40, 8), (5, 5))
 
 
+_imported = None
+
+
 def _package():
-    """The framework's package: its parent folder is not a package itself."""
-    parent = str(Path.cwd() / "vllm-oxide_amd")
-    if parent not in sys.path:
-        sys.path.insert(0, parent)
-    import oxide_paged_kv
-    return oxide_paged_kv
+    """The framework's package, imported at the first call: its parent folder is not a package itself."""
+    global _imported
+    if _imported is None:
+        parent = str(Path.cwd() / "vllm-oxide_amd")
+        if parent not in sys.path:
+            sys.path.insert(0, parent)
+        import oxide_paged_kv
+        _imported = oxide_paged_kv
+    return _imported
 
 
 def _metadata(name, batch, new_lo, new_hi, ctx_lo, ctx_hi, page, axes=1):
