@@ -84,7 +84,8 @@ class Case:
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,Hq,Hkv,D", [(1, 1, 1, 64), (1, 16, 16, 128), (4, 32, 8, 128), (23, 28, 4, 64), (3, 5, 5, 128),
-                                        (2, 34, 2, 64), (70, 8, 8, 64)])
+                                        (2, 34, 2, 64), (70, 8, 8, 64), (40, 32, 8, 128), (64, 32, 32, 128),
+                                        (64, 64, 32, 128)])
 def test_decode(device, B, Hq, Hkv, D, dtype):
     c = Case(device, B + Hq, dtype, D, Hq, Hkv, [1] * B, behind=0)
     if B > 2:

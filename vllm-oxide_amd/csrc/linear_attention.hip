@@ -5,10 +5,12 @@
 // No reference counterpart: every layer of its models is softmax attention.
 //
 // linear_decode: one token.  Bound by HBM, the state read and written once (8 D^2 bytes
-// a head against 4 D^2 + 2 G D^2 operations).  A workgroup holds kCols columns of one
+// a head against 4 D^2 + 2 G D^2 operations).  A workgroup holds COLS columns of one
 // state in registers -- out's columns need S's columns only -- so nothing is joined
 // between workgroups; the sum over the key dimension goes over the lanes that share a
-// column, then over the waves through LDS.
+// column, then over the waves through LDS.  Heads run fastest in the grid, so that with
+// kv heads a multiple of the eight XCDs one of them gets all columns of a state: 64
+// sequences on 32 heads at D = 128 (268 MB) 56 -> 52 us.
 #include <math.h>
 
 #include <algorithm>
@@ -77,31 +79,32 @@ struct DecaySteps {
 };
 
 constexpr int kDecodeThreads = 256;
-constexpr int kDecodeCols = 32;  // state columns of a workgroup
 
 // One token with the state's columns in registers: s[i] are 4 columns of key row
-// i * kRows + row.  q (G heads) and k are in LDS as fp32.  Writes G x kDecodeCols
-// outputs.
-template <class Tag, int D>
+// i * kRows + row.  ONCE: the states pass through the caches without a claim on them.
+template <class Tag, int D, int COLS, bool ONCE>
 __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) {
-  constexpr int kLanes = kDecodeCols / 4;           // lanes of a row's columns
+  constexpr int kLanes = COLS / 4;                  // lanes of a row's columns
   constexpr int kRows = kDecodeThreads / kLanes;    // rows that the workgroup holds at once
   constexpr int N = D / kRows;
   constexpr int kHeads = 8;  // query heads joined at a time
   __shared__ float s_q[kHeads][D];
-  __shared__ float s_part[kHeads][kDecodeThreads / 64][kDecodeCols];
-  const int slices = D / kDecodeCols;
-  const int slice = blockIdx.x % slices;
-  const int n = blockIdx.x / slices % p.num_kv_heads;
-  const int b = blockIdx.x / slices / p.num_kv_heads;
+  __shared__ float s_part[kHeads][kDecodeThreads / 64][COLS];
+  constexpr int kSlices = D / COLS;
+  const int n = blockIdx.x % p.num_kv_heads;
+  const int slice = blockIdx.x / p.num_kv_heads % kSlices;
+  const int b = blockIdx.x / p.num_kv_heads / kSlices;
   const int64_t slot = p.slots[b];
   if (slot < 0 || slot >= p.num_slots) return;
   const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
-  const int col = slice * kDecodeCols + lane * 4;
+  const int col = slice * COLS + lane * 4;
   float* state = p.state + (slot * p.num_kv_heads + n) * D * D + col;
   floatx4 s[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) s[i] = *reinterpret_cast<const floatx4*>(state + (i * kRows + row) * D);
+  for (int i = 0; i < N; ++i) {
+    const floatx4* at = reinterpret_cast<const floatx4*>(state + (i * kRows + row) * D);
+    s[i] = ONCE ? __builtin_nontemporal_load(at) : *at;
+  }
   const uint16_t* k = p.k + b * p.k_stride + n * D;
   const uint16_t* v = p.v + b * p.v_stride + n * D + col;
   const Decay decay = decay_power(p.log_decay[n], 1);
@@ -113,7 +116,11 @@ __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) 
     const float kk = to_f32(Tag{}, k[i * kRows + row]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kk, vv[e], decay * s[i][e]);
-    *reinterpret_cast<floatx4*>(state + (i * kRows + row) * D) = s[i];
+    floatx4* at = reinterpret_cast<floatx4*>(state + (i * kRows + row) * D);
+    if constexpr (ONCE)
+      __builtin_nontemporal_store(s[i], at);
+    else
+      *at = s[i];
   }
   const int64_t heads0 = static_cast<int64_t>(b) * p.num_heads + n * p.group;
   const uint16_t* q = p.q + b * p.q_stride + n * p.group * D;
@@ -138,12 +145,12 @@ __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) 
         *reinterpret_cast<floatx4*>(&s_part[g][threadIdx.x >> 6][lane * 4]) = sum;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * kDecodeCols; i += kDecodeThreads) {
-      const int g = i / kDecodeCols, c = i % kDecodeCols;
+    for (int i = threadIdx.x; i < heads * COLS; i += kDecodeThreads) {
+      const int g = i / COLS, c = i % COLS;
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kDecodeThreads / 64; ++w) sum += s_part[g][w][c];
-      p.out[(heads0 + g0 + g) * D + slice * kDecodeCols + c] = pack1(Tag{}, sum * p.scale);
+      p.out[(heads0 + g0 + g) * D + slice * COLS + c] = pack1(Tag{}, sum * p.scale);
     }
   }
 }
@@ -988,11 +995,26 @@ extern "C" void linear_attention_decode(void* out, const void* q, const void* k,
   }
   if (batch == 0) return;
   set_heads(p, batch, num_heads, num_kv_heads);
+  // 64 columns a workgroup where it saves more than latency: whole rows at D = 64 (200
+  // sequences on 32 heads 42.6 -> 40.0 us), half as many walks over a group's queries (64
+  // sequences on 32/8 heads of 128 16.5 -> 14.7); else 32, four times as many workgroups for
+  // a small batch as states (4 sequences on 16 heads 4.05 against 4.54).
+  const bool wide = (head_dim == 64 || p.group > 1) && batch * num_kv_heads >= oxide::device_cu_count();
+  // States past half the 256 MB last-level cache are not there any more when they are next
+  // needed: non-temporal (64 sequences on 32 heads, 134 MB of states, 51.7 -> 48.7 us; with 16
+  // sequences, 34 MB, 12.7 -> 14.7).
+  const bool once = batch * num_kv_heads * head_dim * head_dim * 4 >= (int64_t{128} << 20);
   dispatch(dtype, head_dim, [&](auto tag, auto d) {
     using Tag = decltype(tag);
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((linear_decode<Tag, D>), dim3(static_cast<unsigned>(batch * num_kv_heads * (D / kDecodeCols))),
-                       dim3(kDecodeThreads), 0, oxide::as_stream(stream), p);
+    auto launch = [&](auto kernel, int cols) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch * num_kv_heads * (D / cols))), dim3(kDecodeThreads), 0,
+                         oxide::as_stream(stream), p);
+    };
+    if (wide)
+      once ? launch(linear_decode<Tag, D, 64, true>, 64) : launch(linear_decode<Tag, D, 64, false>, 64);
+    else
+      once ? launch(linear_decode<Tag, D, 32, true>, 32) : launch(linear_decode<Tag, D, 32, false>, 32);
   });
   oxide::check_launch();
 }
