@@ -11,8 +11,9 @@
 //
 // A token's block comes from the table where the request held it before the step and
 // from the free list where it is new, so tokens never wait for the table's writers and
-// one launch does both.  Every workgroup scans all requests by itself (up to 1024: four
-// a lane, wave scans joined in LDS) and then serves its share of the tokens and of the
+// one launch does both.  Bound by latency: a round trip for the lengths, the scan, a
+// bisection, a round trip for the block id.  Every workgroup scans all requests by itself
+// (up to 1024: four a lane, wave scans joined in LDS) and then serves its share of the tokens and of the
 // new table entries, finding a token's request by bisection of the prefix sums in LDS.
 // Beyond 1024 requests a first launch of one workgroup writes the prefix sums and the
 // second bisects them in memory.
@@ -23,6 +24,28 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kFusedBatch = 1024;  // requests that every workgroup scans by itself
 constexpr int kScanThreads = 1024;
+
+// Division of 32-bit numbers by one that a launch keeps, as a multiplication and shifts
+// (T. Granlund, P. L. Montgomery, "Division by invariant integers using multiplication",
+// PLDI 1994, figure 4.1); the general divide is ten times the operations, and a scan's
+// lane does four for each request.
+struct Divisor {
+  uint32_t d, m;
+  int shift1, shift2;
+};
+Divisor divisor_of(uint32_t d) {
+  int l = 0;
+  while (l < 32 && (uint64_t{1} << l) < d) ++l;
+  const uint64_t m = ((uint64_t{1} << 32) * ((uint64_t{1} << l) - d)) / d + 1;
+  return Divisor{d, static_cast<uint32_t>(m), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t x, Divisor by) {
+  const uint32_t t = __umulhi(by.m, x);
+  return (t + ((x - t) >> by.shift1)) >> by.shift2;
+}
+__device__ __forceinline__ uint64_t divide(uint64_t x, Divisor by) {
+  return (x >> 32) == 0 ? divide(static_cast<uint32_t>(x), by) : x / by.d;
+}
 
 struct StepParams {
   const uint32_t* context_lens;
@@ -38,17 +61,15 @@ struct StepParams {
   int64_t num_tokens;
   int64_t num_free;
   uint32_t width;
-  uint32_t block_size;
+  Divisor block_size;
   int batch;
   int num_axes;
 };
 
 // Blocks of the first `tokens` tokens that the table has room for.
 __device__ __forceinline__ uint32_t blocks_of(const StepParams& p, uint64_t tokens) {
-  const uint64_t n = (tokens >> 32) == 0
-                         ? static_cast<uint64_t>((static_cast<uint32_t>(tokens) / p.block_size) +
-                                                 (static_cast<uint32_t>(tokens) % p.block_size != 0))
-                         : (tokens + p.block_size - 1) / p.block_size;
+  const uint64_t whole = divide(tokens, p.block_size);
+  const uint64_t n = whole + (whole * p.block_size.d != tokens);
   return static_cast<uint32_t>(min(n, static_cast<uint64_t>(p.width)));
 }
 
@@ -56,9 +77,9 @@ struct Sums {
   uint32_t q, k, n;
 };
 
-// Exclusive prefix sums over the workgroup of each lane's three totals.
+// Exclusive prefix sums over the workgroup of each lane's three totals, and all lanes'.
 template <int THREADS>
-__device__ __forceinline__ Sums scan_totals(Sums own, Sums* s_wave) {
+__device__ __forceinline__ Sums scan_totals(Sums own, Sums* s_wave, Sums& all) {
   Sums acc = own;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -69,31 +90,49 @@ __device__ __forceinline__ Sums scan_totals(Sums own, Sums* s_wave) {
   if (lane == 63) s_wave[wave] = acc;
   __syncthreads();
   acc.q -= own.q, acc.k -= own.k, acc.n -= own.n;
-  for (int w = 0; w < wave; ++w) acc.q += s_wave[w].q, acc.k += s_wave[w].k, acc.n += s_wave[w].n;
+  all = Sums{0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const Sums s = s_wave[w];
+    if (w < wave) acc.q += s.q, acc.k += s.k, acc.n += s.n;
+    all.q += s.q, all.k += s.k, all.n += s.n;
+  }
   return acc;
 }
 
-// Each lane takes a run of requests; put(b, sums) is called with the sums before request
-// b, and once with b = batch.
-template <int THREADS, class Put>
-__device__ __forceinline__ void scan_requests(const StepParams& p, Sums* s_wave, Put put) {
-  const int per = (p.batch + THREADS - 1) / THREADS;
-  const int b0 = min(p.batch, static_cast<int>(threadIdx.x) * per), b1 = min(p.batch, b0 + per);
-  auto add = [&](int b, Sums& s) {
-    const uint32_t c = p.context_lens[b], q = p.query_lens[b];
-    const uint64_t total = static_cast<uint64_t>(c) + q;
-    s.q += q;
-    s.k += static_cast<uint32_t>(total);
-    s.n += blocks_of(p, total) - blocks_of(p, c);
-  };
-  Sums own{0, 0, 0};
-  for (int b = b0; b < b1; ++b) add(b, own);
-  Sums at = scan_totals<THREADS>(own, s_wave);
-  for (int b = b0; b < b1; ++b) {
-    put(b, at);
-    add(b, at);
+// THREADS * PER requests at a time, PER neighbours a lane; put(b, context, sums) is called
+// with the sums before request b, and end(sums) with all requests'.
+template <int THREADS, int PER, class Put, class End>
+__device__ __forceinline__ void scan_requests(const StepParams& p, Sums* s_wave, Put put, End end) {
+  Sums before{0, 0, 0};  // of the rounds so far
+  for (int first = 0; first < p.batch; first += THREADS * PER) {
+    const int b0 = first + static_cast<int>(threadIdx.x) * PER;
+    uint32_t c[PER], q[PER];
+    Sums each[PER], own{0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = p.context_lens[min(b0 + i, p.batch - 1)];
+      q[i] = p.query_lens[min(b0 + i, p.batch - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint64_t total = static_cast<uint64_t>(c[i]) + q[i];
+      each[i] = Sums{q[i], static_cast<uint32_t>(total), blocks_of(p, total) - blocks_of(p, c[i])};
+      if (b0 + i >= p.batch) each[i] = Sums{0, 0, 0};
+      own.q += each[i].q, own.k += each[i].k, own.n += each[i].n;
+    }
+    if (first > 0) __syncthreads();  // the wave totals of the round before are read
+    Sums round;
+    Sums at = scan_totals<THREADS>(own, s_wave, round);
+    at.q += before.q, at.k += before.k, at.n += before.n;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (b0 + i < p.batch) put(b0 + i, c[i], at);
+      at.q += each[i].q, at.k += each[i].k, at.n += each[i].n;
+    }
+    before.q += round.q, before.k += round.k, before.n += round.n;
   }
-  if (b1 == p.batch && (b0 < b1 || threadIdx.x == 0)) put(p.batch, at);
+  if (threadIdx.x == 0) end(before);
 }
 
 // The last request whose prefix sum is at most x (sums: batch + 1 of them, sums[batch] > x).
@@ -107,25 +146,18 @@ __device__ __forceinline__ int request_of(const uint32_t* sums, int batch, uint3
   return lo;
 }
 
-__device__ __forceinline__ void put_token(const StepParams& p, const uint32_t* cu_q, const uint32_t* cu_new, int64_t t,
-                                          uint32_t total) {
+__device__ __forceinline__ void put_token(const StepParams& p, const uint32_t* cu_q, const uint32_t* cu_new,
+                                          const uint32_t* context, int64_t t, uint32_t total) {
   int64_t slot = -1;
   int32_t position = 0;
   if (t < total) {
     const int b = request_of(cu_q, p.batch, static_cast<uint32_t>(t));
-    const uint64_t c = p.context_lens[b];
+    const uint64_t c = context[b];
     const uint64_t pos = c + (static_cast<uint32_t>(t) - cu_q[b]);
     position = static_cast<int32_t>(static_cast<uint32_t>(pos));
     if (p.position_offsets)
       position = static_cast<int32_t>(static_cast<uint32_t>(position) + static_cast<uint32_t>(p.position_offsets[b]));
-    uint64_t block, in_block;
-    if (pos >> 32) {
-      block = pos / p.block_size;
-      in_block = pos % p.block_size;
-    } else {
-      block = static_cast<uint32_t>(pos) / p.block_size;
-      in_block = static_cast<uint32_t>(pos) % p.block_size;
-    }
+    const uint64_t block = divide(pos, p.block_size), in_block = pos - block * p.block_size.d;
     if (block < p.width) {
       const uint32_t held = blocks_of(p, c);
       const uint64_t at = cu_new[b] + (block - held);  // where in the free list a new block is
@@ -135,7 +167,7 @@ __device__ __forceinline__ void put_token(const StepParams& p, const uint32_t* c
       } else if (cu_new[b + 1] <= p.num_free && at < cu_new[b + 1]) {
         id = p.free_blocks + at;
       }
-      if (id) slot = static_cast<int64_t>(*id) * p.block_size + static_cast<int64_t>(in_block);
+      if (id) slot = static_cast<int64_t>(*id) * p.block_size.d + static_cast<int64_t>(in_block);
     }
   }
   p.slots[t] = slot;
@@ -144,24 +176,27 @@ __device__ __forceinline__ void put_token(const StepParams& p, const uint32_t* c
 }
 
 // Tokens, then new table entries, over the whole grid.
-__device__ __forceinline__ void serve(const StepParams& p, const uint32_t* cu_q, const uint32_t* cu_new) {
+__device__ __forceinline__ void serve(const StepParams& p, const uint32_t* cu_q, const uint32_t* cu_new,
+                                      const uint32_t* context) {
   const uint32_t total = cu_q[p.batch];
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t t = first; t < p.num_tokens; t += stride) put_token(p, cu_q, cu_new, t, total);
+  for (int64_t t = first; t < p.num_tokens; t += stride) put_token(p, cu_q, cu_new, context, t, total);
   const int64_t handed = min(static_cast<int64_t>(cu_new[p.batch]), p.num_free);
   for (int64_t n = first; n < handed; n += stride) {
     const int b = request_of(cu_new, p.batch, static_cast<uint32_t>(n));
     if (cu_new[b + 1] > p.num_free) continue;  // the list ends inside this request's blocks
-    const uint32_t entry = blocks_of(p, p.context_lens[b]) + static_cast<uint32_t>(n) - cu_new[b];
+    const uint32_t entry = blocks_of(p, context[b]) + static_cast<uint32_t>(n) - cu_new[b];
     p.block_table[static_cast<int64_t>(b) * p.width + entry] = p.free_blocks[n];
   }
 }
 
+template <int PER>
 __global__ __launch_bounds__(kThreads) void step_metadata_fused(StepParams p) {
-  __shared__ uint32_t s_q[kFusedBatch + 1], s_new[kFusedBatch + 1];
+  constexpr int kMost = kThreads * PER;
+  __shared__ uint32_t s_q[kMost + 1], s_new[kMost + 1], s_context[kMost];
   __shared__ Sums s_wave[kThreads / 64];
-  scan_requests<kThreads>(p, s_wave, [&](int b, const Sums& s) {
+  auto put = [&](int b, const Sums& s) {
     s_q[b] = s.q;
     s_new[b] = s.n;
     if (blockIdx.x == 0) {
@@ -169,21 +204,32 @@ __global__ __launch_bounds__(kThreads) void step_metadata_fused(StepParams p) {
       p.cu_k[b] = s.k;
       p.cu_new[b] = s.n;
     }
-  });
+  };
+  scan_requests<kThreads, PER>(
+      p, s_wave,
+      [&](int b, uint32_t context, const Sums& s) {
+        s_context[b] = context;
+        put(b, s);
+      },
+      [&](const Sums& s) { put(p.batch, s); });
   __syncthreads();
-  serve(p, s_q, s_new);
+  serve(p, s_q, s_new, s_context);
 }
 
 __global__ __launch_bounds__(kScanThreads) void step_metadata_scan(StepParams p) {
   __shared__ Sums s_wave[kScanThreads / 64];
-  scan_requests<kScanThreads>(p, s_wave, [&](int b, const Sums& s) {
+  auto put = [&](int b, const Sums& s) {
     p.cu_q[b] = s.q;
     p.cu_k[b] = s.k;
     p.cu_new[b] = s.n;
-  });
+  };
+  scan_requests<kScanThreads, 4>(
+      p, s_wave, [&](int b, uint32_t, const Sums& s) { put(b, s); }, [&](const Sums& s) { put(p.batch, s); });
 }
 
-__global__ __launch_bounds__(kThreads) void step_metadata_serve(StepParams p) { serve(p, p.cu_q, p.cu_new); }
+__global__ __launch_bounds__(kThreads) void step_metadata_serve(StepParams p) {
+  serve(p, p.cu_q, p.cu_new, p.context_lens);
+}
 
 }  // namespace
 
@@ -217,7 +263,7 @@ extern "C" void build_step_metadata_device(const uint32_t* context_lens, const u
   p.num_tokens = num_tokens;
   p.num_free = num_free_blocks;
   p.width = static_cast<uint32_t>(max_blocks_per_seq);
-  p.block_size = static_cast<uint32_t>(block_size);
+  p.block_size = divisor_of(static_cast<uint32_t>(block_size));
   p.batch = static_cast<int>(batch);
   p.num_axes = static_cast<int>(num_axes);
   hipStream_t s = oxide::as_stream(stream);
@@ -225,7 +271,8 @@ extern "C" void build_step_metadata_device(const uint32_t* context_lens, const u
   const int64_t wgs = (items + kThreads - 1) / kThreads, most = oxide::device_cu_count();
   const dim3 grid(static_cast<unsigned>(wgs < 1 ? 1 : wgs > most ? most : wgs));
   if (batch <= kFusedBatch) {
-    hipLaunchKernelGGL(step_metadata_fused, grid, dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL(batch <= kThreads ? step_metadata_fused<1> : step_metadata_fused<kFusedBatch / kThreads>, grid,
+                       dim3(kThreads), 0, s, p);
   } else {
     hipLaunchKernelGGL(step_metadata_scan, dim3(1), dim3(kScanThreads), 0, s, p);
     hipLaunchKernelGGL(step_metadata_serve, grid, dim3(kThreads), 0, s, p);

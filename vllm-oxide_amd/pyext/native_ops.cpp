@@ -267,6 +267,16 @@ const at::Tensor* rows_tensor(PyObject* o, int64_t* stride) {
   return &t;
 }
 
+// A tensor of `type` and `sizes` at a byte offset of a buffer, sharing its storage: an
+// allocation (or a view through the dispatcher) costs 0.6 us on the host, this 0.1.
+at::Tensor part_of(const at::Tensor& buffer, int64_t offset, at::ScalarType type, at::IntArrayRef sizes) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(),
+                                                          c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  t.unsafeGetTensorImpl()->set_storage_offset(offset / static_cast<int64_t>(c10::elementSize(type)));
+  return t;
+}
+
 // step_metadata(context_lens, query_lens, block_table, free_blocks, num_tokens, block_size,
 //               position_offsets, num_axes)
 //   -> (cu_seqlens_q, cu_seqlens_k, slot_mapping, positions, cu_new_blocks)
@@ -287,10 +297,14 @@ PyObject* step_metadata(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const c10::DeviceGuard guard(ctx->device());
   const int64_t B = ctx->size(0), width = table->size(1), free_n = free_list ? free_list->size(0) : 0;
-  const auto i32 = ctx->options().dtype(at::kInt);
-  at::Tensor cu_q = at::empty({B + 1}, i32), cu_k = at::empty({B + 1}, i32), cu_new = at::empty({B + 1}, i32);
-  at::Tensor slots = at::empty({rows}, i32.dtype(at::kLong));
-  at::Tensor pos = axes ? at::empty({axes, rows}, i32) : at::empty({rows}, i32);
+  // One allocation: slots, positions and the three prefix sums, at multiples of 256 bytes.
+  auto up = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+  const int64_t at_pos = up(rows * 8), at_cu = at_pos + up(rows * 4 * (axes ? axes : 1)), cu_bytes = up((B + 1) * 4);
+  const at::Tensor buffer = bytes_like(*ctx, at_cu + 3 * cu_bytes);
+  at::Tensor slots = part_of(buffer, 0, at::kLong, {rows});
+  at::Tensor pos = axes ? part_of(buffer, at_pos, at::kInt, {axes, rows}) : part_of(buffer, at_pos, at::kInt, {rows});
+  at::Tensor cu_q = part_of(buffer, at_cu, at::kInt, {B + 1}), cu_k = part_of(buffer, at_cu + cu_bytes, at::kInt, {B + 1}),
+             cu_new = part_of(buffer, at_cu + 2 * cu_bytes, at::kInt, {B + 1});
   void* s = stream_of(*ctx);
   const uint32_t* pc = static_cast<const uint32_t*>(ctx->data_ptr());
   const uint32_t* pq = static_cast<const uint32_t*>(query->data_ptr());
