@@ -381,19 +381,21 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 
   // A thread moves granule tid % kGranules of rows tid / kGranules + 16 i of a tile.
   const int tile_row = tid / T::kGranules, tile_at = T::at(tile_row, tid % T::kGranules);
+  // Computed where it is needed: kept in registers, the four tensors' would spill others.
   auto lane_bytes = [&](int64_t stride) {
-    return static_cast<uint32_t>(tile_row) * static_cast<uint32_t>(stride * 2) + tid % T::kGranules * 16;
+    const uint32_t t = fresh_copy(tid);
+    return t / T::kGranules * static_cast<uint32_t>(stride * 2) + t % T::kGranules * 16;
   };
-  const uint32_t q_lane = lane_bytes(p.q_stride), k_lane = lane_bytes(p.k_stride), v_lane = lane_bytes(p.v_stride);
   // Rows from `first` (of the chunk) on hold tokens; in place of those before, row `first`
   // is read, and zeros are stored for k and v.
   struct Granules {
     oxide::u32x4 r[T::kLoads];
   };
-  auto load_tile = [&](const uint16_t* base, int64_t stride, uint32_t at, int64_t row0, int first) {
+  auto load_tile = [&](const uint16_t* base, int64_t stride, int64_t row0, int first) {
     const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
     Granules x;
     if (first == 0) {
+      const uint32_t at = lane_bytes(stride);
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i) x.r[i] = *reinterpret_cast<const oxide::u32x4*>(rows + i * 32 * stride + at);
     } else {
@@ -432,10 +434,10 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   auto first_of = [&](int c) { return c + 1 < chunks ? 0 : chunks * kChunk - (t1 - t0); };
   auto row0_of = [&](int c) { return static_cast<int64_t>(t0) + c * kChunk - first_of(c); };
 
-  Granules rk = load_tile(kn, p.k_stride, k_lane, row0_of(0), first_of(0));
-  Granules rv = load_tile(vn, p.v_stride, v_lane, row0_of(0), first_of(0));
+  Granules rk = load_tile(kn, p.k_stride, row0_of(0), first_of(0));
+  Granules rv = load_tile(vn, p.v_stride, row0_of(0), first_of(0));
   Granules rq{};
-  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, q_lane, row0_of(0), first_of(0));
+  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, row0_of(0), first_of(0));
 
   for (int m = tid; m <= kChunk; m += T::kThreads) {
     const Decay x = decay_power(ld, m);
@@ -497,7 +499,6 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const int rows16 = T::at(lane & 15, lane >> 4), rows32 = T::at(lane & 31, half);
   const int cols0 = columns_at<D>(lane, 0), cols1 = columns_at<D>(lane, 1);
   const int scores16 = T::score_at(lane & 15, half) + ((lane >> 4) & 1) * 8, scores32 = T::score_at(lane & 31, half);
-  const uint32_t out_lane = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
 
   const int in_last = t1 - t0 - (chunks - 1) * kChunk;
   const Decay over_chunk = uniform(Decay{s_power[kChunk], s_power_low[kChunk]});
@@ -538,6 +539,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     // A thread moves the granules of the output tile in whose place it puts the next queries.
     auto store_out = [&](int g) {
       char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+      const uint32_t out_lane = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i) {
         const oxide::u32x4 x = *reinterpret_cast<const oxide::u32x4*>(s_q + tile_at + i * T::kStep);
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         }
 
         if (same || more)
-          rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, q_lane, same ? row0 : next_row0,
+          rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, same ? row0 : next_row0,
                          same ? first : next_first);
 
         // Outputs, transposed: a query (of both halves of the chunk) in each lane, value
@@ -684,7 +686,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           interleave<4, 4, 7>();
           fence_schedule();
         }
-        if (!same && more) rk = load_tile(kn, p.k_stride, k_lane, next_row0, next_first);
+        if (!same && more) rk = load_tile(kn, p.k_stride, next_row0, next_first);
         __syncthreads();
 
         const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
@@ -757,8 +759,8 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 
     fence_schedule();
     if (more) {
-      if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, k_lane, next_row0, next_first);
-      rv = load_tile(vn, p.v_stride, v_lane, next_row0, next_first);
+      if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, next_row0, next_first);
+      rv = load_tile(vn, p.v_stride, next_row0, next_first);
     }
     if (update) {
       const int k0 = fresh_copy(cols0), k1 = fresh_copy(cols1);
