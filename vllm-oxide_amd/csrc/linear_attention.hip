@@ -80,9 +80,33 @@ struct DecaySteps {
 
 constexpr int kDecodeThreads = 256;
 
-// One token with the state's columns in registers: s[i] are 4 columns of key row
-// i * kRows + row.  ONCE: the states pass through the caches without a claim on them.
-template <class Tag, int D, int COLS, bool ONCE>
+// Values that are the same in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(uniform(__float_as_int(x))); }
+__device__ __forceinline__ Decay uniform(Decay d) { return Decay{uniform(d.hi), uniform(d.lo)}; }
+
+// A sequence's slot, rows (at most max_q, and none past the last there is) and whether it
+// starts from zero, and a head's decay: asked for together, before any is looked at.
+struct Sequence {
+  int slot, begin, end;
+  bool fresh;
+  float log_decay;
+};
+__device__ __forceinline__ Sequence sequence_of(const LinearParams& p, int b, int n) {
+  const int slot = p.slots[b];
+  const uint32_t from = p.cu_q[b], to = p.cu_q[b + 1];
+  const uint32_t context = *(p.context_lens ? p.context_lens + b : p.cu_q);
+  const float log_decay = p.log_decay[n];
+  const int64_t begin = min(static_cast<int64_t>(from), p.total_q);
+  const int64_t end = min(min(static_cast<int64_t>(to), p.total_q), begin + p.max_q);
+  return Sequence{uniform(slot), uniform(static_cast<int>(begin)), uniform(static_cast<int>(end)),
+                  p.context_lens && uniform(static_cast<int>(context)) == 0, uniform(log_decay)};
+}
+
+// One token a sequence, or (MANY) a few, with the state's columns in registers: s[i] are 4
+// columns of key row i * kRows + row.  ONCE: the states pass through the caches without a
+// claim on them.
+template <class Tag, int D, int COLS, bool ONCE, bool MANY>
 __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) {
   constexpr int kLanes = COLS / 4;                  // lanes of a row's columns
   constexpr int kRows = kDecodeThreads / kLanes;    // rows that the workgroup holds at once
@@ -94,65 +118,86 @@ __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) 
   const int n = blockIdx.x % p.num_kv_heads;
   const int slice = blockIdx.x / p.num_kv_heads % kSlices;
   const int b = blockIdx.x / p.num_kv_heads / kSlices;
-  const int64_t slot = p.slots[b];
-  if (slot < 0 || slot >= p.num_slots) return;
+  Sequence seq{p.slots[b], b, b + 1, false, p.log_decay[n]};
+  if constexpr (MANY) seq = sequence_of(p, b, n);
+  if (seq.slot < 0 || seq.slot >= p.num_slots || seq.begin >= seq.end) return;
   const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   const int col = slice * COLS + lane * 4;
-  float* state = p.state + (slot * p.num_kv_heads + n) * D * D + col;
+  float* state = p.state + (static_cast<int64_t>(seq.slot) * p.num_kv_heads + n) * D * D + col;
   floatx4 s[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const floatx4* at = reinterpret_cast<const floatx4*>(state + (i * kRows + row) * D);
-    s[i] = ONCE ? __builtin_nontemporal_load(at) : *at;
+    s[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (!MANY || !seq.fresh) s[i] = ONCE ? __builtin_nontemporal_load(at) : *at;
   }
-  const uint16_t* k = p.k + b * p.k_stride + n * D;
-  const uint16_t* v = p.v + b * p.v_stride + n * D + col;
-  const Decay decay = decay_power(p.log_decay[n], 1);
-  float vv[4];
+  auto store_state = [&] {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) vv[e] = to_f32(Tag{}, v[e]);
+    for (int i = 0; i < N; ++i) {
+      floatx4* at = reinterpret_cast<floatx4*>(state + (i * kRows + row) * D);
+      if constexpr (ONCE)
+        __builtin_nontemporal_store(s[i], at);
+      else
+        *at = s[i];
+    }
+  };
+  uint16_t k[N];
+  uint2 v;
+  auto read_token = [&](int t) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float kk = to_f32(Tag{}, k[i * kRows + row]);
+    for (int i = 0; i < N; ++i) k[i] = p.k[t * p.k_stride + n * D + i * kRows + row];
+    v = *reinterpret_cast<const uint2*>(p.v + t * p.v_stride + n * D + col);
+  };
+  read_token(seq.begin);
+  const Decay decay = decay_power(seq.log_decay, 1);
+  for (int t = seq.begin; t < seq.end; ++t) {
+    const float vv[4] = {to_f32(Tag{}, static_cast<uint16_t>(v.x)), to_f32(Tag{}, static_cast<uint16_t>(v.x >> 16)),
+                         to_f32(Tag{}, static_cast<uint16_t>(v.y)), to_f32(Tag{}, static_cast<uint16_t>(v.y >> 16))};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kk, vv[e], decay * s[i][e]);
-    floatx4* at = reinterpret_cast<floatx4*>(state + (i * kRows + row) * D);
-    if constexpr (ONCE)
-      __builtin_nontemporal_store(s[i], at);
-    else
-      *at = s[i];
-  }
-  const int64_t heads0 = static_cast<int64_t>(b) * p.num_heads + n * p.group;
-  const uint16_t* q = p.q + b * p.q_stride + n * p.group * D;
-  for (int g0 = 0; g0 < p.group; g0 += kHeads) {
-    const int heads = min(kHeads, p.group - g0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * D; i += kDecodeThreads) s_q[i / D][i % D] = to_f32(Tag{}, q[g0 * D + i]);
-    __syncthreads();
-    for (int g = 0; g < heads; ++g) {
-      floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < N; ++i) {
+      const float kk = to_f32(Tag{}, k[i]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float qq = s_q[g][i * kRows + row];
+      for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kk, vv[e], decay * s[i][e]);
+    }
+    if (MANY && t + 1 < seq.end) read_token(t + 1);
+    if (!MANY) store_state();
+    const uint16_t* q = p.q + t * p.q_stride + n * p.group * D;
+    uint16_t* out = p.out + (static_cast<int64_t>(t) * p.num_heads + n * p.group) * D + slice * COLS;
+    for (int g0 = 0; g0 < p.group; g0 += kHeads) {
+      const int heads = min(kHeads, p.group - g0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < heads * D; i += kDecodeThreads) s_q[i / D][i % D] = to_f32(Tag{}, q[g0 * D + i]);
+      __syncthreads();
+      for (int g = 0; g < heads; ++g) {
+        floatx4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = fmaf(qq, s[i][e], sum[e]);
+        for (int i = 0; i < N; ++i) {
+          const float qq = s_q[g][i * kRows + row];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] = fmaf(qq, s[i][e], sum[e]);
+        }
+        // Over the lanes that hold the same columns: lanes 8 apart by a rotation of the row
+        // of 16, rows of 16 by exchanging them.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (kLanes == 8)
+            sum[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum[e]), 0x128, 0xf, 0xf, true));
+          sum[e] = sum_over_lane_groups(sum[e]);
+        }
+        if ((threadIdx.x & 63) < kLanes)
+          *reinterpret_cast<floatx4*>(&s_part[g][threadIdx.x >> 6][lane * 4]) = sum;
       }
+      __syncthreads();
+      for (int i = threadIdx.x; i < heads * COLS; i += kDecodeThreads) {
+        const int g = i / COLS, c = i % COLS;
+        float sum = 0.f;
 #pragma unroll
-      for (int m = kLanes; m < 64; m <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], m);
-      if ((threadIdx.x & 63) < kLanes)
-        *reinterpret_cast<floatx4*>(&s_part[g][threadIdx.x >> 6][lane * 4]) = sum;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * COLS; i += kDecodeThreads) {
-      const int g = i / COLS, c = i % COLS;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kDecodeThreads / 64; ++w) sum += s_part[g][w][c];
-      p.out[(heads0 + g0 + g) * D + slice * COLS + c] = pack1(Tag{}, sum * p.scale);
+        for (int w = 0; w < kDecodeThreads / 64; ++w) sum += s_part[g][w][c];
+        out[static_cast<int64_t>(g0 + g) * D + c] = pack1(Tag{}, sum * p.scale);
+      }
     }
   }
+  if (MANY) store_state();
 }
 
 // Prompts, 64 tokens at a time on the matrix cores.  With S the state before a chunk,
@@ -311,34 +356,15 @@ __device__ __forceinline__ float wave_max(float x) {
   return max_over_lane_groups(x);
 }
 
-// Values that are the same in every lane, in scalar registers.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ float uniform(float x) { return __int_as_float(uniform(__float_as_int(x))); }
-__device__ __forceinline__ Decay uniform(Decay d) { return Decay{uniform(d.hi), uniform(d.lo)}; }
-
-// A sequence's slot, rows (at most max_q, and none past the last there is) and whether it
-// starts from zero, and a head's decay: asked for together, before any is looked at.
-struct Sequence {
-  int slot, begin, end;
-  bool fresh;
-  float log_decay;
-};
-__device__ __forceinline__ Sequence sequence_of(const LinearParams& p, int b, int n) {
-  const int slot = p.slots[b];
-  const uint32_t from = p.cu_q[b], to = p.cu_q[b + 1];
-  const uint32_t context = *(p.context_lens ? p.context_lens + b : p.cu_q);
-  const float log_decay = p.log_decay[n];
-  const int64_t begin = min(static_cast<int64_t>(from), p.total_q);
-  const int64_t end = min(min(static_cast<int64_t>(to), p.total_q), begin + p.max_q);
-  return Sequence{uniform(slot), uniform(static_cast<int>(begin)), uniform(static_cast<int>(end)),
-                  p.context_lens && uniform(static_cast<int>(context)) == 0, uniform(log_decay)};
-}
-
 // What a launch does with its pieces of sequences.
 enum Mode {
   kWhole,   // a sequence from its slot's state to its end
-  kSums,    // a piece's own sum, from a zero state, into the workspace; not the last piece's
-  kPieces,  // a piece's outputs, from its begin's state in the workspace
+  // A piece's own sum, from a zero state (the first: from the slot's, which it also copies),
+  // into the workspace; not the last piece's.
+  kSums,
+  // A piece's outputs, from its begin's state in the workspace.  The last piece's writes the
+  // slot, which no other piece reads in this launch.
+  kPieces,
 };
 
 template <class Tag, int D, int MODE>
@@ -453,26 +479,47 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[mt][r] = 0.f;
-  if (MODE != kSums && !seq.fresh && (MODE == kWhole || piece == 0 || !p.joined)) {
+  // The workspace keeps a state as its threads hold it: four registers of all threads, the
+  // next four.
+  auto read_dump = [&](const float* from, auto of) {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
+      for (int r = 0; r < 16; r += 4) {
+        const floatx4 x = *reinterpret_cast<const floatx4*>(from + (mt * 4 + r / 4) * T::kThreads * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[mt][r + e] = of(S[mt][r + e], x[e]);
+      }
+  };
+  auto write_dump = [&](float* to) {
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<floatx4*>(to + (mt * 4 + r / 4) * T::kThreads * 4) =
+            floatx4{S[mt][r], S[mt][r + 1], S[mt][r + 2], S[mt][r + 3]};
+  };
+  // Where a cut sequence's first piece leaves a copy of the slot's state.
+  float* const copy = MODE == kWhole ? nullptr
+                                     : p.workspace + ((p.units + begin / p.piece_tokens) * p.num_kv_heads + n) * D * D + tid * 4;
+  if (piece == 0 && !seq.fresh) {
+    if (MODE == kPieces && !last) {
+      read_dump(copy, [](float, float x) { return x; });
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
+      if (MODE == kSums) write_dump(copy);
+    }
   }
   if (MODE == kPieces && piece > 0 && unit < p.units) {
     // The state at the piece's begin, or the earlier pieces' sums one after the other.
     const Decay over_piece = decay_power(ld, p.piece_tokens);
-    for (int back = p.joined ? 0 : piece - 1; back >= 0; --back) {
-      const float* from = ws - static_cast<int64_t>(back) * p.num_kv_heads * D * D;
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(from + (mt * 4 + r / 4) * T::kThreads * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[mt][r + e] = p.joined ? x[e] : over_piece * S[mt][r + e] + x[e];
-        }
-    }
+    const bool joined = p.joined;
+    for (int back = joined ? 0 : piece - 1; back >= 0; --back)
+      read_dump(ws - static_cast<int64_t>(back) * p.num_kv_heads * D * D,
+                [&](float now, float x) { return joined ? x : over_piece * now + x; });
   }
 
   // Decays of the wave's scores (bf16: with the outputs' scale): query 16 strip + lane % 16,
@@ -828,12 +875,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       for (int r = 0; r < 16; ++r) S[mt][r] *= s_unit;
   }
   if (MODE == kSums) {
-#pragma unroll
-    for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *reinterpret_cast<floatx4*>(ws + (mt * 4 + r / 4) * T::kThreads * 4) =
-            floatx4{S[mt][r], S[mt][r + 1], S[mt][r + 2], S[mt][r + 3]};
+    write_dump(ws);
   } else if (last) {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
@@ -843,11 +885,10 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 }
 
 // The pieces' sums become the states at the next pieces' begins, in place:
-//   start(0) = the slot's state or zero, start(i + 1) = lambda^piece_tokens start(i) + sum(i).
+//   start(1) = sum(0), start(i + 1) = lambda^piece_tokens start(i) + sum(i).
 // A thread carries four values of a state through its sequence's pieces.
 template <int D>
 __global__ __launch_bounds__(256) void linear_prefill_join(LinearParams p) {
-  using T = Tiles<D>;
   constexpr int kQuads = D * D / 4;
   const int blocks = kQuads / 256;
   // Heads run fastest in all three grids: with kv heads a multiple of the eight XCDs, a
@@ -860,16 +901,7 @@ __global__ __launch_bounds__(256) void linear_prefill_join(LinearParams p) {
   if (slot < 0 || slot >= p.num_slots) return;
   const int sums = seq.end > begin ? (seq.end - begin - 1) / p.piece_tokens : 0;  // all pieces but the last
   if (sums == 0 || begin / p.piece_tokens >= p.units) return;
-  // Where the workspace's quad lies in the state (as linear_prefill_chunks keeps it).
-  const int tid = quad % T::kThreads, part = quad / T::kThreads, lane = tid & 63;
-  const int row = 32 * (part / 4) + 16 * (part % 4 / 2) + 8 * (lane >> 5) + 4 * (part % 2);
-  const int col = 32 * (tid >> 6) + deal(lane & 31);
   floatx4 s = {0.f, 0.f, 0.f, 0.f};
-  if (!seq.fresh) {
-    const float* state = p.state + (static_cast<int64_t>(slot) * p.num_kv_heads + n) * D * D + row * D + col;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = state[e * D];
-  }
   const Decay fall = decay_power(seq.log_decay, p.piece_tokens);
   const int64_t first = begin / p.piece_tokens;
   const int count = static_cast<int>(min(static_cast<int64_t>(sums), p.units - first));
@@ -982,6 +1014,38 @@ void set_heads(LinearParams& p, int64_t batch, int64_t num_heads, int64_t num_kv
   p.group = static_cast<int>(num_heads / num_kv_heads);
 }
 
+// Prompts of so few tokens are walked one by one, as single tokens are: against a chunk
+// padded to 64, 4 tokens of one sequence on 16 heads 6.1 for 7.3 us, of 24 on 32/8 heads
+// 11.7 for 13.5, of 64 on 32 heads 40 for 36; 8 tokens 8.9 for 7.3, 20 for 14 and 65 for 36.
+constexpr int kFewTokens = 4;
+
+// One token a sequence, or a few.
+template <bool MANY>
+void launch_tokens(const LinearParams& p, int64_t head_dim, int dtype, hipStream_t s) {
+  const int64_t states = int64_t{p.batch} * p.num_kv_heads;
+  // 64 columns a workgroup where it saves more than latency: whole rows at D = 64 (200
+  // sequences on 32 heads 42.6 -> 40.0 us), half as many walks over a group's queries (64
+  // sequences on 32/8 heads of 128 16.5 -> 14.7); else 32, four times as many workgroups for
+  // a small batch as states (4 sequences on 16 heads 4.05 against 4.54).
+  const bool wide = (head_dim == 64 || p.group > 1) && states >= oxide::device_cu_count();
+  // States past half the 256 MB last-level cache are not there any more when they are next
+  // needed: non-temporal (64 sequences on 32 heads, 134 MB of states, 51.7 -> 48.7 us; with 16
+  // sequences, 34 MB, 12.7 -> 14.7).
+  const bool once = states * head_dim * head_dim * 4 >= (int64_t{128} << 20);
+  dispatch(dtype, head_dim, [&](auto tag, auto d) {
+    using Tag = decltype(tag);
+    constexpr int D = decltype(d)::value;
+    auto launch = [&](auto kernel, int cols) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(states * (D / cols))), dim3(kDecodeThreads), 0,
+                         s, p);
+    };
+    if (wide)
+      once ? launch(linear_decode<Tag, D, 64, true, MANY>, 64) : launch(linear_decode<Tag, D, 64, false, MANY>, 64);
+    else
+      once ? launch(linear_decode<Tag, D, 32, true, MANY>, 32) : launch(linear_decode<Tag, D, 32, false, MANY>, 32);
+  });
+}
+
 }  // namespace
 
 extern "C" void linear_attention_decode(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,
@@ -997,27 +1061,7 @@ extern "C" void linear_attention_decode(void* out, const void* q, const void* k,
   }
   if (batch == 0) return;
   set_heads(p, batch, num_heads, num_kv_heads);
-  // 64 columns a workgroup where it saves more than latency: whole rows at D = 64 (200
-  // sequences on 32 heads 42.6 -> 40.0 us), half as many walks over a group's queries (64
-  // sequences on 32/8 heads of 128 16.5 -> 14.7); else 32, four times as many workgroups for
-  // a small batch as states (4 sequences on 16 heads 4.05 against 4.54).
-  const bool wide = (head_dim == 64 || p.group > 1) && batch * num_kv_heads >= oxide::device_cu_count();
-  // States past half the 256 MB last-level cache are not there any more when they are next
-  // needed: non-temporal (64 sequences on 32 heads, 134 MB of states, 51.7 -> 48.7 us; with 16
-  // sequences, 34 MB, 12.7 -> 14.7).
-  const bool once = batch * num_kv_heads * head_dim * head_dim * 4 >= (int64_t{128} << 20);
-  dispatch(dtype, head_dim, [&](auto tag, auto d) {
-    using Tag = decltype(tag);
-    constexpr int D = decltype(d)::value;
-    auto launch = [&](auto kernel, int cols) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch * num_kv_heads * (D / cols))), dim3(kDecodeThreads), 0,
-                         oxide::as_stream(stream), p);
-    };
-    if (wide)
-      once ? launch(linear_decode<Tag, D, 64, true>, 64) : launch(linear_decode<Tag, D, 64, false>, 64);
-    else
-      once ? launch(linear_decode<Tag, D, 32, true>, 32) : launch(linear_decode<Tag, D, 32, false>, 32);
-  });
+  launch_tokens<false>(p, head_dim, dtype, oxide::as_stream(stream));
   oxide::check_launch();
 }
 
@@ -1025,7 +1069,7 @@ extern "C" size_t linear_attention_prefill_workspace_size(int64_t total_q, int64
                                                           int64_t num_kv_heads, int64_t head_dim,
                                                           int64_t max_seqlen_q) {
   const Plan plan = plan_prefill(total_q, batch, num_heads, num_kv_heads, head_dim, max_seqlen_q);
-  return static_cast<size_t>(plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
+  return static_cast<size_t>(2 * plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
 }
 
 extern "C" void linear_attention_prefill(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,
@@ -1051,8 +1095,13 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
   p.cu_q = cu_seqlens_q;
   p.total_q = total_q;
   p.max_q = static_cast<int>(max_seqlen_q < total_q ? max_seqlen_q : total_q);
+  if (p.max_q <= kFewTokens) {
+    launch_tokens<true>(p, head_dim, dtype, oxide::as_stream(stream));
+    oxide::check_launch();
+    return;
+  }
   const Plan plan = plan_prefill(total_q, batch, num_heads, num_kv_heads, head_dim, max_seqlen_q);
-  const size_t need = static_cast<size_t>(plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
+  const size_t need = static_cast<size_t>(2 * plan.units * num_kv_heads * head_dim * head_dim) * sizeof(float);
   const bool cut = plan.piece_tokens > 0 && workspace && oxide::aligned16(workspace) && workspace_bytes >= need;
   hipStream_t s = oxide::as_stream(stream);
   dispatch(dtype, head_dim, [&](auto tag, auto d) {
