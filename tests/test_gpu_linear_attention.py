@@ -107,7 +107,8 @@ def test_prefill(device, lens, Hq, Hkv, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lens", [[4000], [2500, 1, 700, 0, 3000]], ids=["one", "ragged"])
+@pytest.mark.parametrize("lens", [[4000], [2500, 1, 700, 0, 3000], [3] * 150 + [3000] + [0, 0, 65] * 20 + [1200]],
+                         ids=["one", "ragged", "among many"])
 def test_prefill_of_long_sequences(device, lens, dtype):
     """Long enough that pieces are worked on side by side, with the workspace and without one."""
     import torch
@@ -116,6 +117,24 @@ def test_prefill_of_long_sequences(device, lens, dtype):
         c = Case(device, len(lens), dtype, 128, 4, 2, lens, decays=[0.0, -0.002])
         c.prefill(workspace=given)
         c.check(what="no workspace" if given is not None else "workspace")
+
+
+@pytest.mark.parametrize("longest", [700, 6000])
+def test_a_longest_length_that_is_only_a_bound(device, longest):
+    """A captured step's maximum is its rows, whatever the lengths; the rows may begin behind others."""
+    import oxide_paged_kv as ox
+
+    c = Case(device, 21, "bf16", 128, 2, 2, [600, 10, 90], behind=6000)
+    skip = 77  # rows of nobody
+    cu = c.i32(np.concatenate([[0], np.cumsum(c.lens)]) + skip)
+    ox.linear_attn_prefill(c.q, c.k, c.v, c.ld_t, c.state, c.slots_t, cu, longest, c.scale, context_lens=c.ctx_t,
+                           out=c.out)
+    got = _value(to_bits(c.out), "bf16")
+    q, k, v = (_value(p, "bf16")[skip:skip + 700] for p in c.parts)
+    want, s_want, size, s_size = ref.linear_attention(q, k, v, c.ld, c.start, c.slots, c.lens, c.scale, c.ctx == 0)
+    ref.assert_linear_close(got[skip:skip + 700], want, size, "bf16", 600, "out")
+    ref.assert_linear_close(c.state.cpu().numpy(), s_want, s_size, "f32", 600, "state")
+    assert np.all(got[:skip] == 7.0) and np.all(got[skip + 700:] == 7.0)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -42,7 +42,7 @@ struct LinearParams {
   int64_t num_slots;
   int64_t units;  // states of each kv head in the workspace
   int batch, num_heads, num_kv_heads, group, max_q;
-  int piece_tokens, pieces;  // tokens of a piece, pieces of the longest sequence
+  int piece_tokens;
   bool joined;  // the workspace holds the states at the pieces' begins, not the pieces' sums
   float scale;
 };
@@ -356,6 +356,55 @@ __device__ __forceinline__ float wave_max(float x) {
   return max_over_lane_groups(x);
 }
 
+// The last sequence whose key is at most x, -1 if there is none: every wave by itself, 64
+// sequences at a time.  key(b) grows with b and is computed from the row b starts at.
+template <class Key>
+__device__ __forceinline__ int last_sequence(const LinearParams& p, int x, Key key) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = p.batch;
+  while (true) {
+    const int step = (n + 63) / 64, at = lo + lane * step;
+    bool ok = false;
+    if (lane * step < n) ok = key(at, static_cast<int>(min(static_cast<int64_t>(p.cu_q[at]), p.total_q))) <= x;
+    const int found = __popcll(__ballot(ok));
+    if (found == 0) return -1;
+    lo += (found - 1) * step;
+    n = min(step, n - (found - 1) * step);
+    if (step == 1) return uniform(lo);
+  }
+}
+
+// The sequence and piece at a place of the grid.  Up to 64 sequences have their pieces one
+// after the other, by a scan of their numbers, and the grid's spare places come last (places
+// with nothing to do in between leave compute units idle: 39 -> 48 us for four prompts of
+// 1024 on 16 heads).  More have them from floor(begin / piece_tokens) + b on: no two
+// sequences' are the same and none is past total_q / piece_tokens + batch.
+struct Place {
+  int sequence, piece;
+};
+__device__ __forceinline__ Place place_of(const LinearParams& p, int at) {
+  if (p.batch == 1) return Place{0, at};
+  if (p.batch > 64) {
+    const int b = last_sequence(p, at, [&](int i, int begin) { return begin / p.piece_tokens + i; });
+    if (b < 0) return Place{-1, 0};
+    const int begin = uniform(static_cast<int>(min(static_cast<int64_t>(p.cu_q[b]), p.total_q)));
+    return Place{b, at - b - begin / p.piece_tokens};
+  }
+  const int lane = threadIdx.x & 63;
+  const int64_t begin = min(static_cast<int64_t>(p.cu_q[min(lane, p.batch)]), p.total_q);
+  const int64_t end = min(min(static_cast<int64_t>(p.cu_q[min(lane + 1, p.batch)]), p.total_q), begin + p.max_q);
+  const int own = end > begin ? static_cast<int>((end - begin - 1) / p.piece_tokens) + 1 : 0;
+  int before = own;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int add = __shfl_up(before, off);
+    if (lane >= off) before += add;
+  }
+  before -= own;
+  const int b = __popcll(__ballot(lane < p.batch && before <= at)) - 1;
+  return Place{uniform(b), at - uniform(__shfl(before, max(b, 0)))};
+}
+
 // What a launch does with its pieces of sequences.
 enum Mode {
   kWhole,   // a sequence from its slot's state to its end
@@ -385,14 +434,19 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), half = lane >> 5;
   const int n = blockIdx.x % p.num_kv_heads;
-  const int piece = MODE == kWhole ? 0 : blockIdx.x / p.num_kv_heads % p.pieces;
-  const int b = blockIdx.x / p.num_kv_heads / (MODE == kWhole ? 1 : p.pieces);
+  int piece = 0, b = blockIdx.x / p.num_kv_heads;
+  if constexpr (MODE != kWhole) {
+    const Place at = place_of(p, b);
+    b = at.sequence;
+    piece = at.piece;
+    if (b < 0) return;
+  }
   const Sequence seq = sequence_of(p, b, n);
   const int slot = seq.slot, begin = seq.begin, end = seq.end;
   const float ld = seq.log_decay;
   if (slot < 0 || slot >= p.num_slots) return;
-  const int t0 = begin + (MODE == kWhole ? 0 : min(end - begin, piece * p.piece_tokens));
-  if (t0 >= end) return;
+  if (piece < 0 || begin >= end || piece > (end - begin - 1) / max(p.piece_tokens, 1)) return;
+  const int t0 = begin + (MODE == kWhole ? 0 : piece * p.piece_tokens);
   const int t1 = MODE == kWhole ? end : t0 + min(end - t0, p.piece_tokens);
   const bool last = t1 == end;
   if (MODE == kSums && last) return;
@@ -895,12 +949,16 @@ __global__ __launch_bounds__(256) void linear_prefill_join(LinearParams p) {
   // head's pieces, and with them what the workspace holds of it, stay on one.
   const int n = blockIdx.x % p.num_kv_heads;
   const int quad = blockIdx.x / p.num_kv_heads % blocks * 256 + threadIdx.x;
-  const int b = blockIdx.x / p.num_kv_heads / blocks;
+  // The cut sequence, if there is one, whose first sum is this unit: the last that starts in
+  // its piece_tokens rows.
+  const int unit = blockIdx.x / p.num_kv_heads / blocks;
+  const int b = last_sequence(p, unit, [&](int, int begin) { return begin / p.piece_tokens; });
+  if (b < 0) return;
   const Sequence seq = sequence_of(p, b, n);
   const int slot = seq.slot, begin = seq.begin;
-  if (slot < 0 || slot >= p.num_slots) return;
+  if (slot < 0 || slot >= p.num_slots || begin / p.piece_tokens != unit) return;
   const int sums = seq.end > begin ? (seq.end - begin - 1) / p.piece_tokens : 0;  // all pieces but the last
-  if (sums == 0 || begin / p.piece_tokens >= p.units) return;
+  if (sums == 0) return;
   floatx4 s = {0.f, 0.f, 0.f, 0.f};
   const Decay fall = decay_power(seq.log_decay, p.piece_tokens);
   const int64_t first = begin / p.piece_tokens;
@@ -1116,14 +1174,14 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
     p.workspace = static_cast<float*>(workspace);
     p.units = plan.units;
     p.piece_tokens = static_cast<int>(plan.piece_tokens);
-    p.pieces = static_cast<int>((p.max_q + plan.piece_tokens - 1) / plan.piece_tokens);
-    const dim3 grid(heads * static_cast<unsigned>(p.pieces));
+    const dim3 grid(static_cast<unsigned>((plan.units + batch) * num_kv_heads));
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kSums>), grid, threads, 0, s, p);
     // A piece adds up the sums before it by itself where they are few: over P pieces that
     // reads P (P - 1) / 2 states, where joining first moves 3 (P - 1) and is a launch more.
-    p.joined = p.pieces > 8;
+    p.joined = p.max_q > 8 * plan.piece_tokens;
     if (p.joined)
-      hipLaunchKernelGGL((linear_prefill_join<D>), dim3(heads * (D * D / 4 / 256)), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((linear_prefill_join<D>),
+                         dim3(static_cast<unsigned>(plan.units * num_kv_heads * (D * D / 4 / 256))), dim3(256), 0, s, p);
     hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), grid, threads, 0, s, p);
   });
   oxide::check_launch();
