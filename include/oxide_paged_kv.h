@@ -509,7 +509,7 @@ void build_step_metadata_device(const uint32_t* context_lens, const uint32_t* qu
  *                given twice, which sequence's state it ends with is not defined.
  *
  * q, k, v, out and state have to be 16-byte aligned, the row strides multiples of 8 up to
- * 2^26.
+ * 2^25.
  * Supported: f16/bf16, head_dim 64 or 128, any group.  State and sums are fp32.
  */
 void linear_attention_decode(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,

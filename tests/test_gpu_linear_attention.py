@@ -266,6 +266,20 @@ def test_offsets_past_32_bits(device):
     assert torch.equal(state[slot], c.state[c.slots[0]])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_as_far_apart_as_they_may_be(device, dtype):
+    """The last chunk's rows are 2^26 bytes apart: offsets of almost 2^32."""
+    import torch
+    import oxide_paged_kv as ox
+
+    c = Case(device, 40, dtype, 128, 2, 2, [64 + 61], behind=0)
+    far = torch.empty(125, 1 << 25, dtype=c.q.dtype, device=device)
+    far[:, :6 * 128] = torch.cat([c.q, c.k, c.v], 1).view(125, -1)
+    q, k, v = far[:, :6 * 128].view(125, 6, 128).split([2, 2, 2], 1)
+    ox.linear_attn_prefill(q, k, v, c.ld_t, c.state, c.slots_t, c.cu, 125, c.scale, context_lens=c.ctx_t, out=c.out)
+    c.check()
+
+
 def test_captured_calls_replay(device):
     """A captured prompt and a captured token, replayed between eager work: as eager calls from the same state."""
     import torch

@@ -85,6 +85,14 @@ def test_linear_attention_refuses(call, change, code):
     assert call(**change) == code
 
 
+@pytest.mark.parametrize("call", [_decode, _prefill])
+@pytest.mark.parametrize("stride", ["sq", "sk", "sv"])
+def test_linear_attention_refuses_rows_too_far_apart(call, stride):
+    """64 rows' offsets in bytes have to fit 32 bits."""
+    far = ctypes.c_void_p(1 << 46)  # not between the rows
+    assert call(out=far, **{stride: (1 << 25) + 8}) == INVALID
+
+
 def test_prefill_refuses():
     assert _prefill(cu=None) == INVALID and _prefill(T=-1) == INVALID and _prefill(longest=-1) == INVALID
 

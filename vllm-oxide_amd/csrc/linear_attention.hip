@@ -1005,7 +1005,7 @@ Plan plan_prefill(int64_t total_q, int64_t batch, int64_t num_heads, int64_t num
   return Plan{piece, total_q / piece};
 }
 
-constexpr int64_t kMaxStride = 1 << 26;  // elements: 16 rows' offsets in bytes fit 32 bits
+constexpr int64_t kMaxStride = 1 << 25;  // elements: a chunk's rows' offsets in bytes fit 32 bits
 
 // Argument checks of both entries; OXIDE_OK, or the error to record.
 int check_linear(const LinearParams& p, int64_t rows, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
