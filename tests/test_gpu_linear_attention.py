@@ -208,6 +208,35 @@ def test_nothing_reaches_earlier_tokens(device, part, bad, dtype):
     assert np.all(np.isfinite(state[others])) and np.all(np.isfinite(state[s, 0]))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_other_columns_keep_their_values(device, bad, D, dtype):
+    """An infinity or NaN in one value column, of a token's v or of the state before: the others as without it."""
+    import torch
+
+    bits = {"bf16": {"inf": 0x7F80, "nan": 0x7FC0}, "f16": {"inf": 0x7C00, "nan": 0x7E00}}[dtype][str(bad)]
+    c = Case(device, 41, dtype, D, 2, 1, [150, 90], decays=[-0.01])
+    c.ctx[:] = 100
+    c.ctx_t = c.i32(c.ctx)
+    c.parts[2][70, 0, 5] = bits
+    c.start[c.slots[1], 0, :, 9] = bad
+    c.q, c.k, c.v = to_torch(np.concatenate(c.parts, 1), dtype, device).split([2, 1, 1], 1)
+    c.state.copy_(torch.from_numpy(c.start))
+    c.prefill()
+    got, state = _value(to_bits(c.out), dtype), c.state.double().cpu().numpy()
+    q, k, v = (_value(p, dtype) for p in c.parts)
+    with np.errstate(invalid="ignore"):
+        want, s_want, size, s_size = ref.linear_attention(q, k, v, c.ld, c.start, c.slots, c.lens, c.scale)
+    for rows, column in ((slice(0, 150), 5), (slice(150, 240), 9)):
+        rest = np.arange(D) != column
+        ref.assert_linear_close(got[rows][..., rest], want[rows][..., rest], size[rows][..., rest], dtype, 150, "out")
+    for b, column in enumerate((5, 9)):
+        rest, s = np.arange(D) != column, c.slots[b]
+        ref.assert_linear_close(state[s][..., rest], s_want[s][..., rest], s_size[s][..., rest], "f32", 150, "state")
+    assert not np.isfinite(got[70:150, :, 5]).any() and not np.isfinite(got[150:240, :, 9]).any()
+
+
 def test_fresh_sequences_do_not_read_their_slots(device):
     c = Case(device, 9, "bf16", 64, 2, 2, [70, 5])
     c.ctx[:] = 0

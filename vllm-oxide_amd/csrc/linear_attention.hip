@@ -654,7 +654,8 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     // of two, so the registers hold the state over `s_unit`.
     const bool update = MODE == kSums || more || last;
     Pow2 v_scale{1.f, 1.f};
-    if constexpr (kF16) v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(most)));
+    // An infinity or NaN has no part in the power: other columns keep their values.
+    if constexpr (kF16) v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(min(most, 0x7bff))));
     float fall = 1.f;
     if (update) fall = steps.next(more ? over_chunk : over_last) * (kF16 ? s_unit * v_scale.down : 1.f);
     if constexpr (MODE != kSums) {
@@ -665,7 +666,16 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(S[mt][r]));
-        s_scale = scale_for_f16(wave_max(m));  // of the registers' values
+        m = wave_max(m);
+        if (!(m < INFINITY)) {  // nor here
+          m = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) m = fabsf(S[mt][r]) < INFINITY ? fmaxf(m, fabsf(S[mt][r])) : m;
+          m = wave_max(m);
+        }
+        s_scale = scale_for_f16(m);  // of the registers' values
       }
 
       for (int g = 0; g < p.group; ++g) {
