@@ -536,7 +536,11 @@ void linear_attention_decode(void* out, const void* q, const void* k, const void
  *                walked from its first chunk to its last, with the same results within
  *                rounding.  Calls that share a workspace must not overlap in time.
  *
- * A NaN or infinity in v reaches its own token and later ones, no earlier one.
+ * A NaN or infinity in v reaches its own token and later ones, no earlier one.  A decay of
+ * a head that grows (log_decay > 0) may be up to 0.4 here, and its powers over a sequence's
+ * tokens have to stay in fp32's range: beyond, results may be infinite or NaN before the
+ * single tokens' would be.  In f16 a column's values are held to 2^-38 of the largest of
+ * v in their 64 tokens, and of the state's 32 columns where it is multiplied.
  * Alignment, types and shapes as for linear_attention_decode.
  */
 void linear_attention_prefill(void* out, const void* q, const void* k, const void* v, int64_t q_row_stride,

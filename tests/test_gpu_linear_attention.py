@@ -237,6 +237,20 @@ def test_other_columns_keep_their_values(device, bad, D, dtype):
     assert not np.isfinite(got[70:150, :, 5]).any() and not np.isfinite(got[150:240, :, 9]).any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,growth", [([20, 64], 0.4), ([100, 3], 0.1), ([64, 150], 0.05), ([3000], 0.004)], ids=str)
+def test_states_that_grow(device, lens, growth, dtype):
+    """A decay over 1: weights of up to e^25 in a chunk, of e^12 over pieces; rows padded in front have none."""
+    import torch
+
+    c = Case(device, 42, dtype, 128, 2, 2, lens, decays=[growth, 0.0])
+    c.start *= np.float32(2.0 ** -6)
+    c.state.copy_(torch.from_numpy(c.start))
+    c.scale = math.exp(-growth * max(lens)) / 8  # the largest outputs are a few hundred
+    c.prefill()
+    c.check()
+
+
 def test_fresh_sequences_do_not_read_their_slots(device):
     c = Case(device, 9, "bf16", 64, 2, 2, [70, 5])
     c.ctx[:] = 0

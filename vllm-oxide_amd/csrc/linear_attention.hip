@@ -654,8 +654,11 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     // of two, so the registers hold the state over `s_unit`.
     const bool update = MODE == kSums || more || last;
     Pow2 v_scale{1.f, 1.f};
-    // An infinity or NaN has no part in the power: other columns keep their values.
-    if constexpr (kF16) v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(min(most, 0x7bff))));
+    // An infinity or NaN has no part in the power: other columns keep their values.  A head
+    // whose states grow weighs v by up to lambda^n.
+    if constexpr (kF16)
+      v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(min(most, 0x7bff))) *
+                              fmaxf((more ? over_chunk : over_last).hi, 1.f));
     float fall = 1.f;
     if (update) fall = steps.next(more ? over_chunk : over_last) * (kF16 ? s_unit * v_scale.down : 1.f);
     if constexpr (MODE != kSums) {
