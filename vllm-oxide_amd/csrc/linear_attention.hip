@@ -471,19 +471,20 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   struct Granules {
     oxide::u32x4 r[T::kLoads];
   };
-  auto load_tile = [&](const uint16_t* base, int64_t stride, int64_t row0, int first) {
+  // Without a branch: addresses that two paths agree on are 64-bit registers, and what is
+  // loaded on one path only is waited for with all that was asked for since.
+  auto load_tile = [&](const uint16_t* base, int64_t stride, int64_t row0, int first, auto once) {
     const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
+    const uint32_t step = static_cast<uint32_t>(stride) * 32, at = lane_bytes(stride);
+    const uint32_t least = fresh_copy(tid) % T::kGranules * 16 + static_cast<uint32_t>(first) * static_cast<uint32_t>(stride * 2);
     Granules x;
-    if (first == 0) {
-      const uint32_t at = lane_bytes(stride);
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) x.r[i] = *reinterpret_cast<const oxide::u32x4*>(rows + i * 32 * stride + at);
-    } else {
-#pragma unroll
-      for (int i = 0; i < T::kLoads; ++i)
-        x.r[i] = *reinterpret_cast<const oxide::u32x4*>(
-            rows + (static_cast<uint32_t>(max(16 * i + tile_row, first)) * static_cast<uint32_t>(stride * 2) +
-                    tid % T::kGranules * 16));
+    for (int i = 0; i < T::kLoads; ++i) {
+      const oxide::u32x4* from = reinterpret_cast<const oxide::u32x4*>(rows + max(at + i * step, least));
+      if constexpr (decltype(once)::value)
+        x.r[i] = __builtin_nontemporal_load(from);
+      else
+        x.r[i] = *from;
     }
     return x;
   };
@@ -507,6 +508,10 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     return x;
   };
 
+  // q and out pass through the caches without a claim on them: keys and values are there
+  // when the second launch reads them again.
+  constexpr std::true_type kOnce{};
+  constexpr std::false_type kKeep{};
   const uint16_t* const qn = p.q + static_cast<int64_t>(n) * p.group * D;
   const uint16_t* const kn = p.k + static_cast<int64_t>(n) * D;
   const uint16_t* const vn = p.v + static_cast<int64_t>(n) * D;
@@ -514,10 +519,11 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   auto first_of = [&](int c) { return c + 1 < chunks ? 0 : chunks * kChunk - (t1 - t0); };
   auto row0_of = [&](int c) { return static_cast<int64_t>(t0) + c * kChunk - first_of(c); };
 
-  Granules rk = load_tile(kn, p.k_stride, row0_of(0), first_of(0));
-  Granules rv = load_tile(vn, p.v_stride, row0_of(0), first_of(0));
+  // In the order in which they are asked for later.
   Granules rq{};
-  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, row0_of(0), first_of(0));
+  if constexpr (MODE != kSums) rq = load_tile(qn, p.q_stride, row0_of(0), first_of(0), kOnce);
+  Granules rk = load_tile(kn, p.k_stride, row0_of(0), first_of(0), kKeep);
+  Granules rv = load_tile(vn, p.v_stride, row0_of(0), first_of(0), kKeep);
 
   for (int m = tid; m <= kChunk; m += T::kThreads) {
     const Decay x = decay_power(ld, m);
@@ -606,9 +612,8 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const Decay over_last = uniform(Decay{s_power[in_last], s_power_low[in_last]});
   DecaySteps steps;
   float s_unit = 1.f;
-  for (int c = 0; c < chunks; ++c) {
-    const int first = first_of(c);
-    const int64_t row0 = row0_of(c);
+  // The rows that are in registers, of which the first `first` are padding, into the tiles.
+  auto put_rows = [&](int c, int first) {
     rk = arrived(rk);
     rv = arrived(rv);
     if (first > 0) {
@@ -617,7 +622,6 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     }
     store_tile(s_k, rk);
     store_tile(s_v, rv);
-    if constexpr (MODE != kSums) store_tile(s_q, arrived(rq));
     if constexpr (kF16) {
       u16x2_t most = {0, 0};
 #pragma unroll
@@ -631,28 +635,46 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       for (int i = 0; i < T::kLoads; ++i) zero = add_zeros(__builtin_bit_cast(uint4, rv.r[i]), zero);
       if (zero != zero) s_most[c & 1] = 1;
     }
+  };
+  put_rows(0, first_of(0));
+  if constexpr (MODE != kSums) store_tile(s_q, arrived(rq));
+
+  // All chunks but the last ask for the next one's rows and have no padding.  Rows go into
+  // their tiles in the chunk that asked for them: where a wait for loads may meet paths with
+  // and without them, or with and without later stores, it waits for all of these as well.
+  auto chunk = [&](int c, auto more_constant) __attribute__((always_inline)) {
+    constexpr bool more = decltype(more_constant)::value;
+    const int first = more ? 0 : first_of(c);
+    const int64_t row0 = row0_of(c);
     __syncthreads();
     const int most = uniform(s_most[c & 1]);
     if (tid == 0) s_most[(c + 1) & 1] = 0;  // last read before the barrier that ended chunk c - 1
     // The next chunk's rows are asked for a tile at a time, between the phases of this one: all
     // at once they fill the memory pipe and every wave waits to get its loads into it.
-    const bool more = c + 1 < chunks;
     // A thread moves the granules of the output tile in whose place it puts the next queries.
-    auto store_out = [&](int g) {
-      char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
-      const uint32_t out_lane = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
+    // Padding's threads store row `first` once more.
+    auto read_out = [&] {
+      Granules x;
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) {
-        const oxide::u32x4 x = *reinterpret_cast<const oxide::u32x4*>(s_q + tile_at + i * T::kStep);
-        if (16 * i + tile_row >= first)
-          *reinterpret_cast<oxide::u32x4*>(out + i * 16 * static_cast<int64_t>(p.num_heads * D * 2) + out_lane) = x;
-      }
+      for (int i = 0; i < T::kLoads; ++i)
+        x.r[i] = *reinterpret_cast<const oxide::u32x4*>(
+            s_q + (more || first == 0 ? tile_at + i * T::kStep
+                                      : T::at(max(16 * i + tile_row, first), tid % T::kGranules)));
+      return x;
+    };
+    auto store_out = [&](int g, const Granules& x) {
+      char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+      const uint32_t step = static_cast<uint32_t>(p.num_heads * D) * 32, at = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
+      const uint32_t least = more ? 0 : fresh_copy(tid) % T::kGranules * 16 + static_cast<uint32_t>(first) * (step / 16);
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i)
+        __builtin_nontemporal_store(x.r[i], reinterpret_cast<oxide::u32x4*>(out + max(at + i * step, least)));
     };
     const int next_first = first_of(c + 1);
     const int64_t next_row0 = row0_of(c + 1);
     // The state's decay over the chunk.  f16: what is added to it comes scaled by v's power
     // of two, so the registers hold the state over `s_unit`.
-    const bool update = MODE == kSums || more || last;
+    const bool update = more || MODE == kSums || last;
     Pow2 v_scale{1.f, 1.f};
     // An infinity or NaN has no part in the power: other columns keep their values.  A head
     // whose states grow weighs v by up to lambda^n.
@@ -681,8 +703,8 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         s_scale = scale_for_f16(m);  // of the registers' values
       }
 
-      for (int g = 0; g < p.group; ++g) {
-        const bool same = g + 1 < p.group;  // the next tile of queries is this chunk's
+      auto head = [&](int g, auto same_constant) __attribute__((always_inline)) {
+        constexpr bool same = decltype(same_constant)::value;  // the next tile of queries is this chunk's
         const float fall_now = same ? 1.f : fall;
 
         // Scores: K Q^T tiles, a query in each lane and four keys in its registers.
@@ -746,7 +768,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 
         if (same || more)
           rq = load_tile(same ? qn + (g + 1) * D : qn, p.q_stride, same ? row0 : next_row0,
-                         same ? first : next_first);
+                         same ? first : next_first, kOnce);
 
         // Outputs, transposed: a query (of both halves of the chunk) in each lane, value
         // columns in its registers.  First what the state gives, while other waves' scores
@@ -800,7 +822,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           interleave<4, 4, 7>();
           fence_schedule();
         }
-        if (!same && more) rk = load_tile(kn, p.k_stride, next_row0, next_first);
+        if (!same && more) rk = load_tile(kn, p.k_stride, next_row0, next_first, kKeep);
         __syncthreads();
 
         const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
@@ -864,17 +886,19 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           }
         if (same) {
           __syncthreads();
-          store_out(g);
+          store_out(g, read_out());
           store_tile(s_q, arrived(rq));
           __syncthreads();
         }
-      }
+      };
+      for (int g = 0; g + 1 < p.group; ++g) head(g, std::true_type{});
+      head(p.group - 1, std::false_type{});
     }
 
     fence_schedule();
     if (more) {
-      if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, next_row0, next_first);
-      rv = load_tile(vn, p.v_stride, next_row0, next_first);
+      if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, next_row0, next_first, kKeep);
+      rv = load_tile(vn, p.v_stride, next_row0, next_first, kKeep);
     }
     if (update) {
       const int k0 = fresh_copy(cols0), k1 = fresh_copy(cols1);
@@ -932,8 +956,16 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       if constexpr (kF16) s_unit = v_scale.up;
     }
     __syncthreads();
-    if constexpr (MODE != kSums) store_out(p.group - 1);
-  }
+    Granules x{};
+    if constexpr (MODE != kSums) x = read_out();
+    if constexpr (more) put_rows(c + 1, next_first);
+    if constexpr (MODE != kSums) {
+      store_out(p.group - 1, x);
+      if constexpr (more) store_tile(s_q, arrived(rq));
+    }
+  };
+  for (int c = 0; c + 1 < chunks; ++c) chunk(c, std::true_type{});
+  chunk(chunks - 1, std::false_type{});
 
   if constexpr (kF16) {
 #pragma unroll
