@@ -405,58 +405,54 @@ __device__ __forceinline__ Place place_of(const LinearParams& p, int at) {
   return Place{uniform(b), at - uniform(__shfl(before, max(b, 0)))};
 }
 
-// What a launch does with its pieces of sequences.
+// What a workgroup does with its piece of a sequence.
 enum Mode {
-  kWhole,   // a sequence from its slot's state to its end
+  kWhole,  // a sequence from its slot's state to its end
   // A piece's own sum, from a zero state (the first: from the slot's, which it also copies),
-  // into the workspace; not the last piece's.
+  // into the workspace.
   kSums,
-  // A piece's outputs, from its begin's state in the workspace.  The last piece's writes the
-  // slot, which no other piece reads in this launch.
+  // A piece's outputs, from its begin's state in the workspace.  Its own state is for them
+  // alone: of bf16 it takes v as two values, 16 bits of it.
   kPieces,
+  kLast,  // also the slot's new state, which no other piece reads in this launch
 };
 
-template <class Tag, int D, int MODE>
-__global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(LinearParams p) {
+// OUTPUTS: a kernel that computes them.
+template <int D, bool OUTPUTS>
+struct alignas(16) ChunkTiles {
+  char k[Tiles<D>::kTileBytes], v[Tiles<D>::kTileBytes];
+  char q[OUTPUTS ? Tiles<D>::kTileBytes : 16], p[OUTPUTS ? kChunk * 128 : 16];
+  float weight[kChunk];                            // lambda^(63 - j)
+  float power[kChunk + 1], power_low[kChunk + 1];  // lambda^m, and what its rounding leaves
+  float up[kChunk];                                // f16: 2^e of P's rows
+  // Of even and odd chunks: bf16, whether v holds an infinity or NaN; f16, its largest
+  // magnitude's bits (0x7c00 on: one of those).
+  int most[2];
+};
+
+// Rows t0 .. t1 - 1 of a sequence and kv head n, its piece `piece`.
+template <class Tag, int D, int MODE, class Lds>
+__device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequence& seq, int n, int piece, int t0,
+                                            int t1, Lds& lds) {
   using T = Tiles<D>;
   constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
   constexpr int kMt = D / 32;  // tiles of 32 key rows
-  __shared__ char s_k[T::kTileBytes] __attribute__((aligned(16)));
-  __shared__ char s_v[T::kTileBytes] __attribute__((aligned(16)));
-  __shared__ char s_q[MODE == kSums ? 16 : T::kTileBytes] __attribute__((aligned(16)));
-  __shared__ char s_p[MODE == kSums ? 16 : kChunk * 128] __attribute__((aligned(16)));
-  __shared__ float s_power[kChunk + 1], s_power_low[kChunk + 1];   // lambda^m, and what its rounding leaves
-  __shared__ float s_weight[kChunk] __attribute__((aligned(16)));  // lambda^(63 - j)
-  __shared__ float s_up[kChunk];                                   // f16: 2^e of P's rows
-  // Of even and odd chunks: bf16, whether v holds an infinity or NaN; f16, its largest
-  // magnitude's bits (0x7c00 on: one of those).
-  __shared__ int s_most[2];
-
+  char *const s_k = lds.k, *const s_v = lds.v, *const s_q = lds.q, *const s_p = lds.p;
+  float *const s_weight = lds.weight, *const s_power = lds.power, *const s_power_low = lds.power_low;
+  float* const s_up = lds.up;
+  int* const s_most = lds.most;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), half = lane >> 5;
-  const int n = blockIdx.x % p.num_kv_heads;
-  int piece = 0, b = blockIdx.x / p.num_kv_heads;
-  if constexpr (MODE != kWhole) {
-    const Place at = place_of(p, b);
-    b = at.sequence;
-    piece = at.piece;
-    if (b < 0) return;
-  }
-  const Sequence seq = sequence_of(p, b, n);
-  const int slot = seq.slot, begin = seq.begin, end = seq.end;
   const float ld = seq.log_decay;
-  if (slot < 0 || slot >= p.num_slots) return;
-  if (piece < 0 || begin >= end || piece > (end - begin - 1) / max(p.piece_tokens, 1)) return;
-  const int t0 = begin + (MODE == kWhole ? 0 : piece * p.piece_tokens);
-  const int t1 = MODE == kWhole ? end : t0 + min(end - t0, p.piece_tokens);
-  const bool last = t1 == end;
-  if (MODE == kSums && last) return;
-  // The piece's state in the workspace: every sequence has floor(begin / piece_tokens) ...
-  // on for its own.
-  const int64_t unit = MODE == kWhole ? 0 : begin / p.piece_tokens + piece - (MODE == kPieces ? 1 : 0);
+  // The workspace's states: sums of all pieces but the last, every sequence's from
+  // floor(begin / piece_tokens) on; and `units` behind its first, a copy of the slot's state
+  // that a cut sequence starts from.
+  const int64_t first_unit = MODE == kWhole ? 0 : seq.begin / p.piece_tokens;
+  const int64_t unit = first_unit + piece - (MODE == kPieces || MODE == kLast ? 1 : 0);
   if (MODE == kSums && unit >= p.units) return;
   float* const ws = p.workspace + (unit * p.num_kv_heads + n) * D * D + tid * 4;
+  auto copy = [&] { return p.workspace + ((p.units + first_unit) * p.num_kv_heads + n) * D * D + tid * 4; };
   float* const state =
-      p.state + (static_cast<int64_t>(slot) * p.num_kv_heads + n) * D * D + 32 * wave + deal(lane & 31);
+      p.state + (static_cast<int64_t>(seq.slot) * p.num_kv_heads + n) * D * D + 32 * wave + deal(lane & 31);
   const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
 
   // A thread moves granule tid % kGranules of rows tid / kGranules + 16 i of a tile.
@@ -471,12 +467,11 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   struct Granules {
     oxide::u32x4 r[T::kLoads];
   };
-  // Without a branch: addresses that two paths agree on are 64-bit registers, and what is
-  // loaded on one path only is waited for with all that was asked for since.
+  // Without a branch, of which the addresses would be 64-bit registers of their own.
   auto load_tile = [&](const uint16_t* base, int64_t stride, int64_t row0, int first, auto once) {
     const char* rows = reinterpret_cast<const char*>(base) + row0 * stride * 2;
     const uint32_t step = static_cast<uint32_t>(stride) * 32, at = lane_bytes(stride);
-    const uint32_t least = fresh_copy(tid) % T::kGranules * 16 + static_cast<uint32_t>(first) * static_cast<uint32_t>(stride * 2);
+    const uint32_t least = fresh_copy(tid) % T::kGranules * 16 + first * static_cast<uint32_t>(stride * 2);
     Granules x;
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) {
@@ -559,21 +554,18 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         *reinterpret_cast<floatx4*>(to + (mt * 4 + r / 4) * T::kThreads * 4) =
             floatx4{S[mt][r], S[mt][r + 1], S[mt][r + 2], S[mt][r + 3]};
   };
-  // Where a cut sequence's first piece leaves a copy of the slot's state.
-  float* const copy = MODE == kWhole ? nullptr
-                                     : p.workspace + ((p.units + begin / p.piece_tokens) * p.num_kv_heads + n) * D * D + tid * 4;
   if (piece == 0 && !seq.fresh) {
-    if (MODE == kPieces && !last) {
-      read_dump(copy, [](float, float x) { return x; });
+    if (MODE == kPieces) {
+      read_dump(copy(), [](float, float x) { return x; });
     } else {
 #pragma unroll
       for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[mt][r] = state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D];
-      if (MODE == kSums) write_dump(copy);
+      if (MODE == kSums) write_dump(copy());
     }
   }
-  if (MODE == kPieces && piece > 0 && unit < p.units) {
+  if ((MODE == kPieces || MODE == kLast) && piece > 0 && unit < p.units) {
     // The state at the piece's begin, or the earlier pieces' sums one after the other.
     const Decay over_piece = decay_power(ld, p.piece_tokens);
     const bool joined = p.joined;
@@ -610,8 +602,10 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   const int in_last = t1 - t0 - (chunks - 1) * kChunk;
   const Decay over_chunk = uniform(Decay{s_power[kChunk], s_power_low[kChunk]});
   const Decay over_last = uniform(Decay{s_power[in_last], s_power_low[in_last]});
+  const float carries[2] = {s_power[(lane & 31) + 1], s_power[(lane & 31) + 33]};  // without padding
   DecaySteps steps;
   float s_unit = 1.f;
+
   // The rows that are in registers, of which the first `first` are padding, into the tiles.
   auto put_rows = [&](int c, int first) {
     rk = arrived(rk);
@@ -649,32 +643,30 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
     __syncthreads();
     const int most = uniform(s_most[c & 1]);
     if (tid == 0) s_most[(c + 1) & 1] = 0;  // last read before the barrier that ended chunk c - 1
-    // The next chunk's rows are asked for a tile at a time, between the phases of this one: all
-    // at once they fill the memory pipe and every wave waits to get its loads into it.
     // A thread moves the granules of the output tile in whose place it puts the next queries.
-    // Padding's threads store row `first` once more.
     auto read_out = [&] {
       Granules x;
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i)
-        x.r[i] = *reinterpret_cast<const oxide::u32x4*>(
-            s_q + (more || first == 0 ? tile_at + i * T::kStep
-                                      : T::at(max(16 * i + tile_row, first), tid % T::kGranules)));
+        x.r[i] = *reinterpret_cast<const oxide::u32x4*>(s_q + tile_at + i * T::kStep);
       return x;
     };
     auto store_out = [&](int g, const Granules& x) {
       char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
-      const uint32_t step = static_cast<uint32_t>(p.num_heads * D) * 32, at = lane_bytes(static_cast<int64_t>(p.num_heads) * D);
-      const uint32_t least = more ? 0 : fresh_copy(tid) % T::kGranules * 16 + static_cast<uint32_t>(first) * (step / 16);
+      const int64_t stride = static_cast<int64_t>(p.num_heads) * D;
+      const uint32_t at = lane_bytes(stride), step = static_cast<uint32_t>(stride) * 32;
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i)
-        __builtin_nontemporal_store(x.r[i], reinterpret_cast<oxide::u32x4*>(out + max(at + i * step, least)));
+        if (more || 16 * i + tile_row >= first)
+          __builtin_nontemporal_store(x.r[i], reinterpret_cast<oxide::u32x4*>(out + (at + i * step)));
     };
+    // The next chunk's rows are asked for a tile at a time, between the phases of this one: all
+    // at once they fill the memory pipe and every wave waits to get its loads into it.
     const int next_first = first_of(c + 1);
     const int64_t next_row0 = row0_of(c + 1);
     // The state's decay over the chunk.  f16: what is added to it comes scaled by v's power
     // of two, so the registers hold the state over `s_unit`.
-    const bool update = more || MODE == kSums || last;
+    constexpr bool update = more || MODE != kPieces;
     Pow2 v_scale{1.f, 1.f};
     // An infinity or NaN has no part in the power: other columns keep their values.  A head
     // whose states grow weighs v by up to lambda^n.
@@ -682,7 +674,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       v_scale = scale_for_f16(to_f32(Tag{}, static_cast<uint16_t>(min(most, 0x7bff))) *
                               fmaxf((more ? over_chunk : over_last).hi, 1.f));
     float fall = 1.f;
-    if (update) fall = steps.next(more ? over_chunk : over_last) * (kF16 ? s_unit * v_scale.down : 1.f);
+    if constexpr (update) fall = steps.next(more ? over_chunk : over_last) * (kF16 ? s_unit * v_scale.down : 1.f);
     if constexpr (MODE != kSums) {
       Pow2 s_scale{1.f, 1.f};
       if constexpr (kF16) {
@@ -790,6 +782,8 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
         };
         uint4 s16[2];
         auto pack_state = [&](int mt) {
+          // Not kept packed from head to head, in 32 more registers.
+          asm volatile("" : "+v"(S[mt]));
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             float x[8];
@@ -823,13 +817,14 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           fence_schedule();
         }
         if (!same && more) rk = load_tile(kn, p.k_stride, next_row0, next_first, kKeep);
-        __syncthreads();
-
         const int v0 = fresh_copy(cols0), v1 = fresh_copy(cols1);
         uint4 v[4], ps[2][4];
 #pragma unroll
+        for (int kb = 0; kb < 4; ++kb) v[kb] = columns_operand<D>(s_v, v0, v1, kb, wave);
+        __syncthreads();
+
+#pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          v[kb] = columns_operand<D>(s_v, v0, v1, kb, wave);
 #pragma unroll
           for (int it = kb / 2; it < 2; ++it) ps[it][kb] = lds_read16(s_p + (p32 ^ (kb << 5)) + it * 32 * 128);
         }
@@ -837,7 +832,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
           const int query = 32 * it + (lane & 31);
-          float carry = s_power[max(query + 1 - first, 0)];
+          float carry = more ? carries[it] : s_power[max(query + 1 - first, 0)];
           if constexpr (kF16) {
             p_scale[it].up = s_up[query];
             p_scale[it].down = __uint_as_float(0x7f000000u - __float_as_uint(p_scale[it].up));  // 1 / 2^e
@@ -900,7 +895,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
       if constexpr (MODE == kSums) rk = load_tile(kn, p.k_stride, next_row0, next_first, kKeep);
       rv = load_tile(vn, p.v_stride, next_row0, next_first, kKeep);
     }
-    if (update) {
+    if constexpr (update) {
       const int k0 = fresh_copy(cols0), k1 = fresh_copy(cols1);
       if constexpr (MODE == kSums) {
 #pragma unroll
@@ -909,7 +904,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
           for (int r = 0; r < 16; ++r) S[mt][r] *= fall;
       }
       // The products of 16 tokens, while the next 16's operands are read and weighted.
-      constexpr int kTerms = kF16 ? 2 : 3;
+      constexpr int kTerms = kF16 || MODE == kPieces ? 2 : 3;
       uint4 term[kTerms], k[kMt];
       auto weigh = [&](uint4 v, int kb) {
         float x[8], y[8];
@@ -966,6 +961,7 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   };
   for (int c = 0; c + 1 < chunks; ++c) chunk(c, std::true_type{});
   chunk(chunks - 1, std::false_type{});
+  if (MODE == kPieces) return;
 
   if constexpr (kF16) {
 #pragma unroll
@@ -975,11 +971,37 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   }
   if (MODE == kSums) {
     write_dump(ws);
-  } else if (last) {
+  } else {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) state[(32 * mt + 16 * (r / 8) + 8 * half + r % 8) * D] = S[mt][r];
+  }
+}
+
+template <class Tag, int D, int MODE>
+__global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(LinearParams p) {
+  __shared__ ChunkTiles<D, MODE != kSums> lds;
+  const int n = blockIdx.x % p.num_kv_heads;
+  int piece = 0, b = blockIdx.x / p.num_kv_heads;
+  if constexpr (MODE != kWhole) {
+    const Place at = place_of(p, b);
+    b = at.sequence;
+    piece = at.piece;
+    if (b < 0) return;
+  }
+  const Sequence seq = sequence_of(p, b, n);
+  const int begin = seq.begin, end = seq.end;
+  if (seq.slot < 0 || seq.slot >= p.num_slots) return;
+  if (piece < 0 || begin >= end || piece > (end - begin - 1) / max(p.piece_tokens, 1)) return;
+  if constexpr (MODE == kWhole) {
+    walk_chunks<Tag, D, kWhole>(p, seq, n, 0, begin, end, lds);
+  } else {
+    const int t0 = begin + piece * p.piece_tokens, t1 = t0 + min(end - t0, p.piece_tokens);
+    if (t1 < end)
+      walk_chunks<Tag, D, MODE>(p, seq, n, piece, t0, t1, lds);
+    else if constexpr (MODE == kPieces)
+      walk_chunks<Tag, D, kLast>(p, seq, n, piece, t0, t1, lds);
   }
 }
 
