@@ -10,7 +10,9 @@
 // between workgroups; the sum over the key dimension goes over the lanes that share a
 // column, then over the waves through LDS.  Heads run fastest in the grid, so that with
 // kv heads a multiple of the eight XCDs one of them gets all columns of a state: 64
-// sequences on 32 heads at D = 128 (268 MB) 56 -> 52 us.
+// sequences on 32 heads at D = 128 (268 MB) 56 -> 52 us, and with the choices of
+// launch_tokens 46.8 (5.78 TB/s, above the rate of a copy that writes as much as it
+// reads, 5.4 at this size).  4 sequences on 16 heads (8.4 MB) take 4.3 us: a launch.
 #include <math.h>
 
 #include <algorithm>
@@ -226,6 +228,18 @@ __global__ __launch_bounds__(kDecodeThreads) void linear_decode(LinearParams p) 
 //
 // v is used for every earlier row of a chunk as 0 * v, which is NaN for an infinity or
 // NaN: a chunk that holds one adds its products one by one instead.
+//
+// Few sequences on few heads leave most of the chip idle, so long ones are cut into pieces:
+// a launch for the pieces' sums, one that joins many of them, one for the outputs.  That
+// reads k and v twice (the second time largely from the last-level cache), and moves a
+// state of 4 D^2 bytes three to five times a piece.
+//
+// What bounds it: the chunk's chain of phases (scores, barrier, outputs, sums, barrier) at
+// the two waves that 256 registers leave a SIMD.  Of its cycles at D = 128 the matrix cores
+// are busy for 28 % and the vector units for 31 %; with all rows read from the caches the
+// kernels take about five sixths of the time.  1 x 8192 tokens on 32 heads (268 MB in and
+// out, 55 us at the rate of a copy) 97.4 us, its kernels 35 + 13 + 53 one by one; 4 x 4096
+// in f16 163 us; 100 tokens on 16 heads 9.7 us, 2 chunks.
 constexpr int kChunk = 64;
 
 template <int D>
@@ -1140,8 +1154,8 @@ void set_heads(LinearParams& p, int64_t batch, int64_t num_heads, int64_t num_kv
 }
 
 // Prompts of so few tokens are walked one by one, as single tokens are: against a chunk
-// padded to 64, 4 tokens of one sequence on 16 heads 6.1 for 7.3 us, of 24 on 32/8 heads
-// 11.7 for 13.5, of 64 on 32 heads 40 for 36; 8 tokens 8.9 for 7.3, 20 for 14 and 65 for 36.
+// padded to 64, 4 tokens of one sequence on 16 heads 6.2 for 7.0 us, of 24 on 32/8 heads
+// 11.6 for 12.5, of 64 on 32 heads 40 for 38; 8 tokens 8.9 for 6.7, 20 for 13 and 65 for 37.
 constexpr int kFewTokens = 4;
 
 // One token a sequence, or a few.

@@ -13,10 +13,12 @@
 // from the free list where it is new, so tokens never wait for the table's writers and
 // one launch does both.  Bound by latency: a round trip for the lengths, the scan, a
 // bisection, a round trip for the block id.  Every workgroup scans all requests by itself
-// (up to 1024: four a lane, wave scans joined in LDS) and then serves its share of the tokens and of the
-// new table entries, finding a token's request by bisection of the prefix sums in LDS.
-// Beyond 1024 requests a first launch of one workgroup writes the prefix sums and the
-// second bisects them in memory.
+// (up to 1024: four a lane, wave scans joined in LDS) and then serves its share of the
+// tokens and of the new table entries, finding a token's request by bisection of the
+// prefix sums in LDS.  64 single tokens 3.7 us, 700 requests with 63k tokens 6.3, of which
+// a launch is 2-3; what is read and written would take 0.3 us.  Beyond 1024 requests a
+// first launch of one workgroup writes the prefix sums and the second bisects them in
+// memory (60,000 requests 93 us).
 #include "oxide_common.hpp"
 
 namespace {
