@@ -1076,11 +1076,15 @@ Plan plan_prefill(int64_t total_q, int64_t batch, int64_t num_heads, int64_t num
     return whole;
   // As many pieces as workgroups are resident (LDS and registers hold two on a compute unit
   // at D = 128, four at 64), but none whose rows are fewer bytes than its state costs
-  // (written, joined, read: 16 D^2, against 4 D (1 + group) a token).
-  const int64_t resident = (head_dim == 128 ? 2 : 4) * oxide::device_cu_count();
-  const int64_t group = num_heads / num_kv_heads;
-  int64_t piece = (total_q * num_kv_heads + resident - 1) / resident;
-  piece = std::max(piece, 4 * head_dim / (1 + group));
+  // (written, joined, read: 16 D^2, against 4 D (1 + group) a token), unless compute units
+  // are left without one: 512 tokens on 16 heads 28 us whole, 18.7 in pieces of 64, 1000 on
+  // 32/8 in f16 35.2 -> 25.2, 2048 on 8 31.9 -> 25.2 (2048 on 32, a piece for each at 256:
+  // 39.9, at 128 47).  Nor more than 32 for that of a sequence, whose join is a chain: 8192
+  // on 2 heads 36.8 us in 32 pieces, 45.7 in 128.
+  const int64_t cus = oxide::device_cu_count(), resident = (head_dim == 128 ? 2 : 4) * cus;
+  const int64_t group = num_heads / num_kv_heads, rows = total_q * num_kv_heads;
+  int64_t piece = std::max((rows + cus - 1) / cus, (std::min(max_seqlen_q, total_q) + 31) / 32);
+  piece = std::max(std::min(piece, 4 * head_dim / (1 + group)), (rows + resident - 1) / resident);
   piece = (piece + kChunk - 1) / kChunk * kChunk;
   if (max_seqlen_q <= 2 * piece) return whole;
   return Plan{piece, total_q / piece};
