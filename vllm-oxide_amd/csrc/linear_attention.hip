@@ -45,6 +45,7 @@ struct LinearParams {
   int64_t units;  // states of each kv head in the workspace
   int batch, num_heads, num_kv_heads, group, max_q;
   int piece_tokens;
+  int part_heads;  // query heads of a kv head that a workgroup takes, where they are dealt out
   bool joined;  // the workspace holds the states at the pieces' begins, not the pieces' sums
   float scale;
 };
@@ -444,10 +445,11 @@ struct alignas(16) ChunkTiles {
   int most[2];
 };
 
-// Rows t0 .. t1 - 1 of a sequence and kv head n, its piece `piece`.
+// Rows t0 .. t1 - 1 of a sequence and kv head n, its piece `piece`; outputs for `heads` query
+// heads of n's, from g0 on (the first workgroup's write the state).
 template <class Tag, int D, int MODE, class Lds>
 __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequence& seq, int n, int piece, int t0,
-                                            int t1, Lds& lds) {
+                                            int t1, int g0, int heads, Lds& lds) {
   using T = Tiles<D>;
   constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
   constexpr int kMt = D / 32;  // tiles of 32 key rows
@@ -521,7 +523,8 @@ __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequenc
   // when the second launch reads them again.
   constexpr std::true_type kOnce{};
   constexpr std::false_type kKeep{};
-  const uint16_t* const qn = p.q + static_cast<int64_t>(n) * p.group * D;
+  const int64_t h0 = static_cast<int64_t>(n) * p.group + g0;
+  const uint16_t* const qn = p.q + h0 * D;
   const uint16_t* const kn = p.k + static_cast<int64_t>(n) * D;
   const uint16_t* const vn = p.v + static_cast<int64_t>(n) * D;
   // Chunk c is rows row0(c) + 0..63 of which the first first(c) are padding.
@@ -666,7 +669,7 @@ __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequenc
       return x;
     };
     auto store_out = [&](int g, const Granules& x) {
-      char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + n * p.group + g) * D);
+      char* const out = reinterpret_cast<char*>(p.out + (row0 * p.num_heads + h0 + g) * D);
       const int64_t stride = static_cast<int64_t>(p.num_heads) * D;
       const uint32_t at = lane_bytes(stride), step = static_cast<uint32_t>(stride) * 32;
 #pragma unroll
@@ -900,8 +903,8 @@ __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequenc
           __syncthreads();
         }
       };
-      for (int g = 0; g + 1 < p.group; ++g) head(g, std::true_type{});
-      head(p.group - 1, std::false_type{});
+      for (int g = 0; g + 1 < heads; ++g) head(g, std::true_type{});
+      head(heads - 1, std::false_type{});
     }
 
     fence_schedule();
@@ -969,7 +972,7 @@ __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequenc
     if constexpr (MODE != kSums) x = read_out();
     if constexpr (more) put_rows(c + 1, next_first);
     if constexpr (MODE != kSums) {
-      store_out(p.group - 1, x);
+      store_out(heads - 1, x);
       if constexpr (more) store_tile(s_q, arrived(rq));
     }
   };
@@ -985,7 +988,7 @@ __device__ __forceinline__ void walk_chunks(const LinearParams& p, const Sequenc
   }
   if (MODE == kSums) {
     write_dump(ws);
-  } else {
+  } else if (g0 == 0) {
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
@@ -1009,13 +1012,23 @@ __global__ __launch_bounds__(Tiles<D>::kThreads, 2) void linear_prefill_chunks(L
   if (seq.slot < 0 || seq.slot >= p.num_slots) return;
   if (piece < 0 || begin >= end || piece > (end - begin - 1) / max(p.piece_tokens, 1)) return;
   if constexpr (MODE == kWhole) {
-    walk_chunks<Tag, D, kWhole>(p, seq, n, 0, begin, end, lds);
+    walk_chunks<Tag, D, kWhole>(p, seq, n, 0, begin, end, 0, p.group, lds);
   } else {
     const int t0 = begin + piece * p.piece_tokens, t1 = t0 + min(end - t0, p.piece_tokens);
+    int g0 = 0, heads = p.group;
+    if constexpr (MODE == kPieces) {
+      // A sequence that is not cut starts from its slot, which the workgroup that writes it
+      // has to have for itself.
+      if (piece > 0 || t1 < end) {
+        g0 = static_cast<int>(blockIdx.y) * p.part_heads;
+        heads = min(p.part_heads, p.group - g0);
+      }
+      if (heads <= 0 || (blockIdx.y > 0 && g0 == 0)) return;
+    }
     if (t1 < end)
-      walk_chunks<Tag, D, MODE>(p, seq, n, piece, t0, t1, lds);
+      walk_chunks<Tag, D, MODE>(p, seq, n, piece, t0, t1, g0, heads, lds);
     else if constexpr (MODE == kPieces)
-      walk_chunks<Tag, D, kLast>(p, seq, n, piece, t0, t1, lds);
+      walk_chunks<Tag, D, kLast>(p, seq, n, piece, t0, t1, g0, heads, lds);
   }
 }
 
@@ -1267,7 +1280,12 @@ extern "C" void linear_attention_prefill(void* out, const void* q, const void* k
     if (p.joined)
       hipLaunchKernelGGL((linear_prefill_join<D>),
                          dim3(static_cast<unsigned>(plan.units * num_kv_heads * (D * D / 4 / 256))), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), grid, threads, 0, s, p);
+    // Query heads of one kv head are dealt out to workgroups, each with the state for itself,
+    // where there are compute units without one.
+    const int64_t idle = oxide::device_cu_count() / std::max<int64_t>(plan.units * num_kv_heads, 1);
+    p.part_heads = static_cast<int>(p.group / std::clamp<int64_t>(idle, 1, p.group));
+    const dim3 parts(grid.x, static_cast<unsigned>((p.group + p.part_heads - 1) / p.part_heads));
+    hipLaunchKernelGGL((linear_prefill_chunks<Tag, D, kPieces>), parts, threads, 0, s, p);
   });
   oxide::check_launch();
 }
