@@ -119,6 +119,15 @@ def test_prefill_of_long_sequences(device, lens, dtype):
         c.check(what="no workspace" if given is not None else "workspace")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hq,Hkv,D", [(20, 4, 128), (7, 1, 64), (33, 3, 64)])
+def test_heads_of_a_group_on_several_workgroups(device, Hq, Hkv, D, dtype):
+    """Few pieces: a group's query heads are dealt out, not always evenly; short sequences are not cut."""
+    c = Case(device, 43, dtype, D, Hq, Hkv, [2000, 70, 500], decays=np.linspace(-0.01, 0, Hkv))
+    c.prefill()
+    c.check()
+
+
 @pytest.mark.parametrize("longest", [700, 6000])
 def test_a_longest_length_that_is_only_a_bound(device, longest):
     """A captured step's maximum is its rows, whatever the lengths; the rows may begin behind others."""
